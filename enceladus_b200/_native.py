@@ -17,11 +17,12 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libenc_b200.so"
 
 # enc_status
-OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_DEVICE_WAIT, ERR_NO_MEMORY = range(6)
+OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_DEVICE_WAIT, ERR_NO_MEMORY, ERR_BAD_INDEX = range(7)
 # enc_dtype
 F32, F16, BF16, I32, I8, I16, I64, U8 = range(8)
 # enc_kernel
-K_SOFTMAX, K_LAYERNORM, K_RMSNORM, K_GELU, K_MATMUL, K_ATTENTION, K_HISTOGRAM, K_CUMSUM, K_ADD, K_MATMUL_INT = range(10)
+(K_SOFTMAX, K_LAYERNORM, K_RMSNORM, K_GELU, K_MATMUL, K_ATTENTION, K_HISTOGRAM, K_CUMSUM, K_ADD, K_MATMUL_INT, K_APPEND_KV,
+ K_PAGED_ATTENTION, K_LOGITS) = range(13)
 VARIANT_AUTO = -1
 
 
@@ -41,6 +42,15 @@ class DeviceInfo(C.Structure):
     _fields_ = [("device", C.c_int), ("sm_count", C.c_int), ("cc_major", C.c_int),
                 ("cc_minor", C.c_int), ("max_smem_per_block", C.c_int), ("l2_bytes", C.c_int),
                 ("global_mem", C.c_uint64), ("name", C.c_char * 128)]
+
+
+class PagedCache(C.Structure):
+    """`enc_paged_cache`: a paged key-value cache and its block table, as the native entry points take it."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("block_table", C.c_void_p),
+                *((n, C.c_int64) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "num_seqs", "table_width", "stride_table",
+                                           "k_stride_page", "k_stride_head", "k_stride_token",
+                                           "v_stride_page", "v_stride_head", "v_stride_token"))]
 
 
 _p, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -66,10 +76,14 @@ SIGNATURES: dict[str, list] = {
     "enc_matmul": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _p],
     "enc_matmul_int": [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _p],
     "enc_attention_fwd": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f, _i, _i, _i, _p],
+    "enc_append_kv": [C.POINTER(PagedCache)] + [_p] * 8 + [_i64] * 3 + [_i] + [_i64] * 10 + [_i, _i, _p],
+    "enc_paged_attention": [C.POINTER(PagedCache), _p, _p, _p, _p] + [_i64] * 5 + [_f, _i64, _p, _i64, _i, _i, _p],
+    "enc_paged_attention_work_bytes": [C.POINTER(PagedCache), _i64, _i, _i],
+    "enc_penalize_logits": [_p, _p] + [_i64] * 4 + [_p, _i64, _i64] + [_p] * 7 + [_i64, _i64, _p, _i64, _i, _i, _p],
     "enc_test_fail_next": [_i],
     "enc_test_device_wait": [C.c_uint, _p],
 }
-_RESTYPES = {"enc_last_error": C.c_char_p, "enc_test_fail_next": None}
+_RESTYPES = {"enc_last_error": C.c_char_p, "enc_test_fail_next": None, "enc_paged_attention_work_bytes": C.c_int64}
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,194 @@
+// Appending keys and values to a paged cache, queries and keys rotated by their positions on the way.
+//
+// Mathematics: each pair (a, b) of a rotated head becomes (a cos - b sin, b cos + a sin) in float32, rounded once; the
+// rest of the head and the values are copied.  The cosines and sines come from float32 tables made once by the caller, so
+// far positions lose nothing to an angle computed in 32 bits.
+//
+// What bounds it: bytes.  Every element is read once and written once, and a token of 32 query and 2 x 8 key-value heads of
+// 128 16-bit elements is 24 KB of traffic against 0.5 KB of table: one CTA per token, a thread keeps one place inside the
+// head (and its cosines and sines in registers) and walks over the heads.
+#include "paged.cuh"
+
+namespace enc {
+namespace {
+
+constexpr int THREADS = 128;
+
+struct AppendArgs {
+    const void *k, *v, *q;
+    void *q_out, *k_cache, *v_cache;
+    const float *cos, *sin;
+    const int32_t *seq_ids, *positions, *block_table;
+    int64_t sk_t, sk_h, sv_t, sv_h, sq_t, sq_h, so_t, so_h, s_cos;
+    int64_t ck_p, ck_h, ck_t, cv_p, cv_h, cv_t, s_table;
+    int64_t num_seqs, num_pages, num_positions, capacity;
+    int q_heads, kv_heads, head_dim, rot_dim;
+    FastDiv page_size;
+};
+
+// One CTA per token.  VEC: 16-byte vectors (NV elements); else single elements.  An item is one place inside a head: a pair
+// of vectors that turn together (one vector of neighbouring pairs when INTERLEAVED), or a vector that is copied.
+template <typename T, bool VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
+    constexpr int NV = VEC ? Pack<T>::N : (INTERLEAVED ? 2 : 1);  // elements of an item's vector
+    constexpr int UN = 4;                                         // heads in flight per thread
+    constexpr int NC = INTERLEAVED ? (NV / 2 > 0 ? NV / 2 : 1) : NV;  // angles of an item
+    struct alignas(VEC ? 16 : sizeof(T)) Vec { T e[NV]; };
+    grid_dependency_wait();
+    const int64_t t = blockIdx.x;
+    const int seq = a.seq_ids[t], pos = a.positions[t];
+    const int turning = INTERLEAVED ? a.rot_dim / NV : a.rot_dim / 2 / NV;
+    const int tail = a.head_dim - a.rot_dim;  // copied elements behind the rotated ones
+    constexpr int CV = VEC ? NV : 1;          // elements of a copied vector
+    const int items = turning + tail / CV;
+    const int x = threadIdx.x % (items < THREADS ? items : THREADS);
+    const int y = threadIdx.x / (items < THREADS ? items : THREADS), ny = items < THREADS ? THREADS / items : 1;
+    const int heads = a.kv_heads + (a.q ? a.q_heads : 0);  // key heads first, then query heads
+
+    bool ok = seq >= 0;
+    int64_t page = 0;
+    int row = 0;
+    if (ok) {
+        ok = seq < a.num_seqs && pos >= 0 && pos < a.capacity && (a.rot_dim == 0 || pos < a.num_positions);
+        if (ok) {
+            const uint32_t pi = a.page_size.div((uint32_t)pos);
+            row = pos - (int)(pi * a.page_size.d);
+            page = a.block_table[seq * a.s_table + pi];
+            ok = page >= 0 && page < a.num_pages;
+        }
+        if (!ok && threadIdx.x == 0) atomicExch(&g_bad_index, 1u);
+    }
+    if (!ok) return;
+
+    const T *k = reinterpret_cast<const T *>(a.k) + t * a.sk_t, *v = reinterpret_cast<const T *>(a.v) + t * a.sv_t;
+    const T *q = reinterpret_cast<const T *>(a.q) + t * a.sq_t;
+    T *qo = reinterpret_cast<T *>(a.q_out) + t * a.so_t;
+    T *kc = reinterpret_cast<T *>(a.k_cache) + page * a.ck_p + row * a.ck_t;
+    T *vc = reinterpret_cast<T *>(a.v_cache) + page * a.cv_p + row * a.cv_t;
+
+    if (y < ny) {
+        for (int it = x; it < items; it += THREADS) {
+            const bool turn = it < turning;
+            const int off = turn ? it * NV : a.rot_dim + (it - turning) * CV, off2 = off + a.rot_dim / 2;
+            float cs[NC], sn[NC];
+            if (turn) {
+                const float *c = a.cos + pos * a.s_cos + it * NC, *s = a.sin + pos * a.s_cos + it * NC;
+#pragma unroll
+                for (int e = 0; e < NC; ++e) {
+                    cs[e] = c[e];
+                    sn[e] = s[e];
+                }
+            }
+            for (int h0 = y; h0 < heads; h0 += ny * UN) {
+                Vec u[UN], w[UN];
+#pragma unroll
+                for (int j = 0; j < UN; ++j) {
+                    const int h = h0 + j * ny;
+                    if (h >= heads) continue;
+                    const T *src = h < a.kv_heads ? k + h * a.sk_h : q + (h - a.kv_heads) * a.sq_h;
+                    if (VEC || turn) u[j] = *reinterpret_cast<const Vec *>(src + off);
+                    else u[j].e[0] = src[off];
+                    if (!INTERLEAVED && turn) w[j] = *reinterpret_cast<const Vec *>(src + off2);
+                }
+#pragma unroll
+                for (int j = 0; j < UN; ++j) {
+                    const int h = h0 + j * ny;
+                    if (h >= heads) continue;
+                    T *dst = h < a.kv_heads ? kc + h * a.ck_h : qo + (h - a.kv_heads) * a.so_h;
+                    if (turn) {
+#pragma unroll
+                        for (int e = 0; e < NC; ++e) {
+                            T &lo = INTERLEAVED ? u[j].e[(2 * e) % NV] : u[j].e[e];
+                            T &hi = INTERLEAVED ? u[j].e[(2 * e + 1) % NV] : w[j].e[e];
+                            const float fa = to_f32(lo), fb = to_f32(hi);
+                            lo = from_f32<T>(fmaf(fa, cs[e], -(fb * sn[e])));
+                            hi = from_f32<T>(fmaf(fb, cs[e], fa * sn[e]));
+                        }
+                        *reinterpret_cast<Vec *>(dst + off) = u[j];
+                        if (!INTERLEAVED) *reinterpret_cast<Vec *>(dst + off2) = w[j];
+                    } else if (VEC) {
+                        *reinterpret_cast<Vec *>(dst + off) = u[j];
+                    } else {
+                        dst[off] = u[j].e[0];
+                    }
+                }
+            }
+        }
+    }
+    // values: plain copies
+    const int vh = a.head_dim / CV, n = a.kv_heads * vh;
+    struct alignas(VEC ? 16 : sizeof(T)) Copy { T e[CV]; };
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const int h = i / vh, c = (i - h * vh) * CV;
+        *reinterpret_cast<Copy *>(vc + h * a.cv_h + c) = *reinterpret_cast<const Copy *>(v + h * a.sv_h + c);
+    }
+}
+
+template <typename T>
+int launch_append(const AppendArgs &a, int64_t tokens, bool interleaved, bool vec, cudaStream_t st) {
+    const dim3 grid((unsigned)tokens);
+    note_indexed_launch();
+    if (vec && interleaved) launch_overlapped(append_kernel<T, true, true>, grid, dim3(THREADS), 0, st, a);
+    else if (vec) launch_overlapped(append_kernel<T, true, false>, grid, dim3(THREADS), 0, st, a);
+    else if (interleaved) launch_overlapped(append_kernel<T, false, true>, grid, dim3(THREADS), 0, st, a);
+    else launch_overlapped(append_kernel<T, false, false>, grid, dim3(THREADS), 0, st, a);
+    return check_launch("enc_append_kv");
+}
+
+}  // namespace
+
+unsigned int take_bad_index_append() { return take_bad_index_word(); }
+int append_variants() { return 1; }
+void append_variant_info(int, char *out, size_t n) { snprintf(out, n, "one CTA of %d threads per token", THREADS); }
+
+}  // namespace enc
+
+extern "C" int enc_append_kv(const enc_paged_cache *cache, const void *k, const void *v, const void *q, void *q_out,
+                             const float *cos, const float *sin, const int32_t *seq_ids, const int32_t *positions,
+                             int64_t tokens, int64_t q_heads, int64_t rot_dim, int interleaved, int64_t num_positions,
+                             int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
+                             int64_t q_stride_token, int64_t q_stride_head, int64_t o_stride_token, int64_t o_stride_head,
+                             int64_t stride_cos, int dtype, int variant, void *stream) {
+    ENC_PROLOGUE();
+    using namespace enc;
+    const char *me = "enc_append_kv";
+    if (!cache) return fail(ENC_ERR_BAD_ARG, "%s: NULL cache", me);
+    if (!is_float_dtype(dtype)) return fail(ENC_ERR_BAD_ARG, "%s: dtype %d is not float16, bfloat16 or float32", me, dtype);
+    if (variant >= append_variants()) return fail(ENC_ERR_BAD_ARG, "%s: variant %d out of range", me, variant);
+    const int bad = check_cache(*cache, me);
+    if (bad) return bad;
+    if (tokens < 0 || q_heads < 0) return fail(ENC_ERR_BAD_ARG, "%s: negative size", me);
+    if (rot_dim < 0 || rot_dim > cache->head_dim || rot_dim % 2) return fail(ENC_ERR_BAD_ARG, "%s: rot_dim %lld must be even and at most head_dim %lld", me, (long long)rot_dim, (long long)cache->head_dim);
+    if ((q != nullptr) != (q_out != nullptr)) return fail(ENC_ERR_BAD_ARG, "%s: q and q_out go together", me);
+    if (tokens == 0) return ENC_OK;
+    if (tokens > 0x7fffffffLL || q_heads > 0xffff) return fail(ENC_ERR_UNSUPPORTED, "%s: more than 2^31-1 tokens or 65535 query heads", me);
+    if (!k || !v || !seq_ids || !positions) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
+    if (rot_dim > 0 && (!cos || !sin)) return fail(ENC_ERR_BAD_ARG, "%s: rot_dim %lld without cos and sin", me, (long long)rot_dim);
+    // (with no pages or no sequences nothing can be in range: the kernel reports every token that is not padding)
+    if ((!cache->k || !cache->v || !cache->block_table) && cache->num_pages > 0 && cache->num_seqs > 0 && cache->table_width > 0)
+        return fail(ENC_ERR_BAD_ARG, "%s: NULL cache tensor", me);
+    AppendArgs a{};
+    a.k = k; a.v = v; a.q = q; a.q_out = q_out; a.k_cache = cache->k; a.v_cache = cache->v;
+    a.cos = cos; a.sin = sin; a.seq_ids = seq_ids; a.positions = positions; a.block_table = cache->block_table;
+    a.sk_t = k_stride_token; a.sk_h = k_stride_head; a.sv_t = v_stride_token; a.sv_h = v_stride_head;
+    a.sq_t = q_stride_token; a.sq_h = q_stride_head; a.so_t = o_stride_token; a.so_h = o_stride_head; a.s_cos = stride_cos;
+    a.ck_p = cache->k_stride_page; a.ck_h = cache->k_stride_head; a.ck_t = cache->k_stride_token;
+    a.cv_p = cache->v_stride_page; a.cv_h = cache->v_stride_head; a.cv_t = cache->v_stride_token;
+    a.s_table = cache->stride_table;
+    a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.num_positions = num_positions;
+    a.capacity = paged_capacity(*cache);
+    a.q_heads = (int)q_heads; a.kv_heads = (int)cache->kv_heads; a.head_dim = (int)cache->head_dim; a.rot_dim = (int)rot_dim;
+    a.page_size = FastDiv((uint32_t)cache->page_size);
+    // 16-byte vectors where every row starts on 16 bytes and no vector straddles the rotated part or its halves
+    const int nv = 16 / (int)dtype_size(dtype);
+    bool vec = cache->head_dim % nv == 0 && rot_dim % (interleaved ? nv : 2 * nv) == 0 && aligned16(k) && aligned16(v) &&
+               aligned16(cache->k) && aligned16(cache->v) && (!q || (aligned16(q) && aligned16(q_out)));
+    for (int64_t s : {a.sk_t, a.sk_h, a.sv_t, a.sv_h, a.ck_p, a.ck_h, a.ck_t, a.cv_p, a.cv_h, a.cv_t}) vec = vec && s % nv == 0;
+    if (q) for (int64_t s : {a.sq_t, a.sq_h, a.so_t, a.so_h}) vec = vec && s % nv == 0;
+    cudaStream_t st = as_stream(stream);
+    switch (dtype) {
+        case ENC_F16: return launch_append<__half>(a, tokens, interleaved != 0, vec, st);
+        case ENC_BF16: return launch_append<__nv_bfloat16>(a, tokens, interleaved != 0, vec, st);
+        default: return launch_append<float>(a, tokens, interleaved != 0, vec, st);
+    }
+}

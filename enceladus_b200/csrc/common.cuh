@@ -29,6 +29,9 @@ struct DeviceProps {
 };
 const DeviceProps &device_props();  // cached per current device
 
+// Tells enc_synchronize that a kernel which checks index arrays on the device has been launched on the current device.
+void note_indexed_launch();
+
 // Word 0 of the per-device status block is set by a kernel whose bounded wait ran out.
 unsigned int *device_error_word();  // device pointer (allocated on first use), or nullptr
 

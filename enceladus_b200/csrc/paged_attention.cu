@@ -1,0 +1,491 @@
+// Attention of one new token per sequence over a paged key-value cache, split over the cache's length and joined.
+//
+// Mathematics: for a query row, s_j = q . k_j * sm_scale * log2(e); one pass over the keys keeps the running maximum m, the
+// sum l = sum_j 2^(s_j - m) and O = sum_j 2^(s_j - m) v_j, all float32.  Two pieces (m1, l1, O1), (m2, l2, O2) of a row join
+// to m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m) and the same for O, in any split.  o = O / l,
+// lse = (m + log2 l) ln 2.  A piece whose scores are all -inf has m = -inf and counts with weight zero.
+//
+// What bounds it: each key and value is read once and used by the query heads that share it, a handful of operations per
+// byte, so the bound is HBM bandwidth; with few or short sequences, latency.
+//
+// Split: the work is a line of 64-key tiles (sequence by sequence, kv head by kv head), dealt out in equal contiguous
+// runs over a grid that fills the GPU once.  Every CTA finds its run from seq_lens by a scan over the batch, so ragged
+// lengths, one long sequence and many short ones all load every SM alike, and nothing about the lengths has to reach
+// the host.  A row that ends inside a run is finished there; the up to two pieces of a run that belong to rows cut by
+// its ends go to a workspace and a second, overlapped launch joins them in order (no atomics: the result does not depend
+// on timing).
+#include "paged.cuh"
+
+namespace enc {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int THREADS = 128, WARPS = THREADS / 32;
+constexpr int TILE = 64;          // keys of a tile
+constexpr int MAX_HEAD_DIM = 256;
+
+struct PagedArgs {
+    const void *q, *k, *v;
+    void *o;
+    float *lse;
+    const int32_t *block_table, *seq_lens;
+    int4 *headers;   // per CTA: the row group that its last piece begins {first query row, rows, last CTA of it, -}
+    float *slots;    // per CTA two pieces of `rows` x (head_dim + 2) floats: O, m, l
+    int64_t sq_s, sq_h, so_s, so_h, sk_p, sk_h, sk_t, sv_p, sv_h, sv_t, s_table;
+    int64_t num_seqs, num_pages, capacity, window;
+    int q_heads, head_dim, group, row_groups;  // query rows per kv head; row groups (of the kernel's row count) per kv head
+    int units;                                 // row groups per sequence: kv_heads * row_groups
+    int min_run;                               // tiles a run has at least
+    float scale;                               // sm_scale * log2(e)
+    FastDiv page_size;
+};
+
+// ---- schedule ------------------------------------------------------------------------------------
+// Keys of sequence b that its row looks at: the first key and how many.
+__device__ __forceinline__ int keys_of(const PagedArgs &a, int64_t b, int &first) {
+    int n = a.seq_lens[b];
+    if (n < 0 || n > a.capacity) {
+        atomicExch(&g_bad_index, 1u);
+        n = n < 0 ? 0 : (int)a.capacity;
+    }
+    first = a.window > 0 && n > a.window ? n - (int)a.window : 0;
+    return n - first;
+}
+__device__ __forceinline__ int64_t tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
+
+struct Run {
+    int64_t seq, at;      // first sequence, first tile inside the sequence's units
+    int64_t begin, end;   // tiles on the line
+    int64_t run;          // tiles of a full run
+};
+
+// Every thread of the CTA returns the CTA's run of tiles.  The sequences are dealt to the threads in contiguous pieces;
+// the thread whose piece holds the run's first tile finds the sequence.
+__device__ __forceinline__ Run find_run(const PagedArgs &a) {
+    __shared__ int64_t warp_total[WARPS], found[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t per = (a.num_seqs + THREADS - 1) / THREADS;
+    const int64_t b0 = threadIdx.x * per, b1 = b0 + per < a.num_seqs ? b0 + per : a.num_seqs;
+    int64_t mine = 0;
+    int first;
+    for (int64_t b = b0; b < b1; ++b) mine += tiles_of(keys_of(a, b, first));
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) warp_total[warp] = upto;
+    __syncthreads();
+    int64_t total = 0, before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += warp_total[w];
+        total += warp_total[w];
+    }
+    total *= a.units;
+    Run r;
+    r.run = (total + gridDim.x - 1) / gridDim.x;
+    if (r.run < a.min_run) r.run = a.min_run;
+    r.begin = blockIdx.x * r.run;
+    r.end = r.begin + r.run < total ? r.begin + r.run : total;
+    r.seq = r.at = 0;
+    if (r.begin >= r.end) return r;  // (the same for all threads: begin and end depend on the block alone)
+    if (before * a.units <= r.begin && r.begin < (before + mine) * a.units) {
+        int64_t at = r.begin - before * a.units;
+        for (int64_t b = b0; b < b1; ++b) {
+            const int64_t t = tiles_of(keys_of(a, b, first)) * a.units;
+            if (at < t) {
+                found[0] = b;
+                found[1] = at;
+                break;
+            }
+            at -= t;
+        }
+    }
+    __syncthreads();
+    r.seq = found[0];
+    r.at = found[1];
+    return r;
+}
+
+__device__ __forceinline__ float *slot_of(const PagedArgs &a, int64_t cta, int which, int rows) {
+    return a.slots + (2 * cta + which) * rows * (int64_t)(a.head_dim + 2);
+}
+
+// A piece's rows, one partial result per warp in shared memory (O unnormalised [WARPS][ROWS][stride], m and l [WARPS][ROWS]),
+// joined and written: to the output when the piece is the whole row, to `slot` otherwise.
+template <typename T, int ROWS>
+__device__ __forceinline__ void write_piece(const PagedArgs &a, const float *so, int stride, const float (*sm)[ROWS], const float (*sl)[ROWS],
+                                            int rows, int64_t seq, int first_head, float *slot) {
+    T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s;
+    for (int i = threadIdx.x; i < rows * a.head_dim; i += THREADS) {
+        const int r = i / a.head_dim, d = i - r * a.head_dim;
+        float m = sm[0][r];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) m = fmaxf(m, sm[w][r]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float c = fast_exp2(sm[w][r] - base);
+            l = fmaf(sl[w][r], c, l);
+            x = fmaf(so[(w * ROWS + r) * stride + d], c, x);
+        }
+        if (slot) {
+            slot[r * (a.head_dim + 2) + d] = x;
+            if (d == 0) {
+                slot[r * (a.head_dim + 2) + a.head_dim] = m;
+                slot[r * (a.head_dim + 2) + a.head_dim + 1] = l;
+            }
+        } else {
+            o[(first_head + r) * a.so_h + d] = from_f32<T>(l == 0.0f ? 0.0f : __fdiv_rn(x, l));
+            if (d == 0 && a.lse) a.lse[seq * a.q_heads + first_head + r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+        }
+    }
+}
+
+// Walks over the CTA's run: process(seq, kv head, first query head, rows, first key, keys, tile range, slot or NULL) per
+// piece.  Also writes the header that the join reads, and the rows of sequences without keys.
+template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk_run(const PagedArgs &a, F process) {
+    const Run run = find_run(a);
+    if (threadIdx.x == 0 && a.headers) a.headers[blockIdx.x].y = 0;
+    int64_t seq = run.seq, at = run.at;
+    for (int64_t pos = run.begin; pos < run.end;) {
+        int first;
+        const int keys = keys_of(a, seq, first);
+        const int64_t tiles = tiles_of(keys);
+        if (at >= tiles * a.units) {
+            at -= tiles * a.units;  // (zero: a sequence's tiles are walked to their end)
+            ++seq;
+            continue;
+        }
+        const int unit = (int)(at / tiles), t0 = (int)(at - unit * tiles);
+        const int t1 = tiles - t0 < run.end - pos ? (int)tiles : t0 + (int)(run.end - pos);
+        const int kv_head = unit / a.row_groups, rg = unit - kv_head * a.row_groups;
+        const int rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
+        const int first_head = kv_head * a.group + rg * ROWS;
+        float *slot = nullptr;
+        if (t0 > 0) {
+            slot = slot_of(a, blockIdx.x, 0, ROWS);
+        } else if (t1 < tiles) {
+            slot = slot_of(a, blockIdx.x, 1, ROWS);
+            if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), (int)((pos + tiles - 1) / run.run), 0);
+        }
+        process(seq, kv_head, first_head, rows, first, keys, t0, t1, slot);
+        pos += t1 - t0;
+        at += t1 - t0;
+    }
+    T *o = reinterpret_cast<T *>(a.o);
+    for (int64_t b = blockIdx.x; b < a.num_seqs; b += gridDim.x) {  // rows without keys
+        int first;
+        if (keys_of(a, b, first) > 0) continue;
+        for (int i = threadIdx.x; i < a.q_heads * a.head_dim; i += THREADS) {
+            const int h = i / a.head_dim, d = i - h * a.head_dim;
+            o[b * a.so_s + h * a.so_h + d] = from_f32<T>(0.0f);
+            if (d == 0 && a.lse) a.lse[b * a.q_heads + h] = -INFINITY;
+        }
+    }
+}
+
+// Where key `pos` of sequence seq lives: its page and its row in it; false (and the error word) if the page is out of range.
+__device__ __forceinline__ bool locate(const PagedArgs &a, int64_t seq, int pos, int64_t &page, int &row) {
+    const uint32_t pi = a.page_size.div((uint32_t)pos);
+    row = pos - (int)(pi * a.page_size.d);
+    page = a.block_table[seq * a.s_table + pi];
+    if (page >= 0 && page < a.num_pages) return true;
+    atomicExch(&g_bad_index, 1u);
+    return false;
+}
+
+// ---- join ------------------------------------------------------------------------------------------
+// One CTA per (run, row): where a run's last piece begins a row group, the pieces of that group are that piece and the first
+// pieces of the runs after it.  Two passes over the pieces' statistics (maximum, then weights), then the weighted sum.
+template <typename T, int ROWS> __global__ void __launch_bounds__(THREADS) join_kernel(PagedArgs a) {
+    __shared__ float red[WARPS], part[WARPS][MAX_HEAD_DIM];
+    grid_dependency_wait();
+    const int4 h = a.headers[blockIdx.x];
+    const int rows = h.y & 255, first_head = h.y >> 8, r = blockIdx.y;
+    if (r >= rows) return;
+    const int n = h.z - (int)blockIdx.x + 1;  // pieces
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t stride = a.head_dim + 2;
+    auto piece = [&](int i) { return slot_of(a, blockIdx.x + i, i == 0 ? 1 : 0, ROWS) + r * stride; };
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, piece(i)[a.head_dim]);
+    m = warp_max(m);
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, red[w]);
+    __syncthreads();
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, x[MAX_HEAD_DIM / 32];
+#pragma unroll
+    for (int i = 0; i < MAX_HEAD_DIM / 32; ++i) x[i] = 0.0f;
+    for (int i = warp; i < n; i += WARPS) {  // a warp takes every WARPS-th piece, its lanes the elements
+        const float *p = piece(i);
+        const float c = fast_exp2(p[a.head_dim] - base);
+        l = fmaf(p[a.head_dim + 1], c, l);
+#pragma unroll
+        for (int j = 0; j < MAX_HEAD_DIM / 32; ++j)
+            if (lane + 32 * j < a.head_dim) x[j] = fmaf(p[lane + 32 * j], c, x[j]);
+    }
+    if (lane == 0) red[warp] = l;
+#pragma unroll
+    for (int j = 0; j < MAX_HEAD_DIM / 32; ++j)
+        if (lane + 32 * j < a.head_dim) part[warp][lane + 32 * j] = x[j];
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) l += red[w];
+    const int64_t seq = h.x;
+    T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s + (first_head + r) * a.so_h;
+    for (int d = threadIdx.x; d < a.head_dim; d += THREADS) {
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) y += part[w][d];
+        o[d] = from_f32<T>(l == 0.0f ? 0.0f : __fdiv_rn(y, l));
+    }
+    if (threadIdx.x == 0 && a.lse) a.lse[seq * a.q_heads + first_head + r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---- CUDA-core kernel: any head_dim up to 256, any dtype, any strides ----------------------------------
+// Eight lanes share a key, four keys per warp at a time; a lane owns CH groups of four neighbouring elements of the head and
+// keeps its part of q and O for ROWS query rows in registers, with statistics of its own per group of eight lanes.  K and V
+// go straight from memory to registers.
+template <typename T, bool VEC> __device__ __forceinline__ void load4(const T *p, int d, int head_dim, float (&f)[4]) {
+    if (VEC) {
+        if (sizeof(T) == 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(p + d);
+            f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+        } else {
+            struct alignas(8) H { T e[4]; };
+            const H x = *reinterpret_cast<const H *>(p + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = to_f32(x.e[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = d + e < head_dim ? to_f32(p[d + e]) : 0.0f;
+    }
+}
+
+template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bounds__(THREADS) paged_simple_kernel(PagedArgs a) {
+    __shared__ float so[WARPS * ROWS * MAX_HEAD_DIM], sm[WARPS][ROWS], sl[WARPS][ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, sub = lane >> 3;
+    const int D = a.head_dim;
+    grid_dependency_wait();
+    walk_run<T, ROWS>(a, [&](int64_t seq, int kv_head, int first_head, int rows, int first, int keys, int t0, int t1, float *slot) {
+        const T *qb = reinterpret_cast<const T *>(a.q) + seq * a.sq_s, *kb = reinterpret_cast<const T *>(a.k) + kv_head * a.sk_h;
+        const T *vb = reinterpret_cast<const T *>(a.v) + kv_head * a.sv_h;
+        float q[ROWS][CH][4], o[ROWS][CH][4], m[ROWS], l[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int d = (c * 8 + l8) * 4;
+                if (r < rows && d < D) load4<T, VEC>(qb + (first_head + r) * a.sq_h, d, D, q[r][c]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    q[r][c][e] = r < rows && d < D ? q[r][c][e] * a.scale : 0.0f;
+                    o[r][c][e] = 0.0f;
+                }
+            }
+        }
+        const int stop = t1 * TILE < keys ? t1 * TILE : keys;
+        for (int j0 = t0 * TILE + warp * 4; j0 < stop; j0 += 4 * WARPS) {  // the same trip count for the whole warp
+            const int j = j0 + sub;
+            int64_t page = 0;
+            int row = 0;
+            const bool in = j < stop && locate(a, seq, first + j, page, row);
+            float k[CH][4], v[CH][4];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int d = (c * 8 + l8) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) k[c][e] = v[c][e] = 0.0f;
+                if (in && d < D) {
+                    load4<T, VEC>(kb + page * a.sk_p + row * a.sk_t, d, D, k[c]);
+                    load4<T, VEC>(vb + page * a.sv_p + row * a.sv_t, d, D, v[c]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                float s = 0.0f;
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s = fmaf(q[r][c][e], k[c][e], s);
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                if (!in) s = -INFINITY;
+                if (s > m[r]) {
+                    const float c0 = m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - s);
+                    m[r] = s;
+                    l[r] *= c0;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[r][c][e] *= c0;
+                }
+                const float p = in ? fast_exp2(s - (m[r] == -INFINITY ? 0.0f : m[r])) : 0.0f;
+                l[r] += p;
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[r][c][e] = fmaf(p, v[c][e], o[r][c][e]);
+            }
+        }
+        // join the four groups of lanes, then hand the warp's result over
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            float mw = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+            mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, 16));
+            const float c0 = fast_exp2(m[r] - (mw == -INFINITY ? 0.0f : mw));
+            float lw = l[r] * c0;
+            lw += __shfl_xor_sync(0xffffffffu, lw, 8);
+            lw += __shfl_xor_sync(0xffffffffu, lw, 16);
+            if (lane == 0) {
+                sm[warp][r] = mw;
+                sl[warp][r] = lw;
+            }
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = o[r][c][e] * c0;
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    const int d = (c * 8 + l8) * 4 + e;
+                    if (sub == 0 && d < D) so[(warp * ROWS + r) * MAX_HEAD_DIM + d] = x;
+                }
+        }
+        __syncthreads();
+        write_piece<T, ROWS>(a, so, MAX_HEAD_DIM, sm, sl, rows, seq, first_head, slot);
+        __syncthreads();
+    });
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+enum { V_CORES = 0, VARIANTS = 1 };
+
+struct Plan {
+    int variant, rows, row_groups, grid;
+    int64_t work;
+};
+
+// Which kernel, how many query rows it takes at a time, how many CTAs, and the bytes for pieces.
+int make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant, Plan &p) {
+    const int group = (int)(q_heads / c.kv_heads);
+    p.variant = V_CORES;
+    p.rows = group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
+    const int per_sm = 4;
+    p.row_groups = (int)cdiv(group, p.rows);
+    const int64_t most = c.num_seqs * c.kv_heads * p.row_groups * cdiv(paged_capacity(c), TILE);  // tiles if every row is full
+    const int64_t fill = (int64_t)device_props().sm_count * per_sm;
+    p.grid = (int)(most < fill ? (most > 0 ? most : 1) : fill);
+    // sequences of one tile are never cut
+    p.work = paged_capacity(c) <= TILE ? 0 : (int64_t)p.grid * 16 + 2 * (int64_t)p.grid * p.rows * (c.head_dim + 2) * 4;
+    return 0;
+}
+
+template <typename T, int CH, int ROWS>
+void launch_simple(const PagedArgs &a, int grid, bool vec, cudaStream_t st) {
+    if (vec) launch_overlapped(paged_simple_kernel<T, CH, ROWS, true>, dim3(grid), dim3(THREADS), 0, st, a);
+    else launch_overlapped(paged_simple_kernel<T, CH, ROWS, false>, dim3(grid), dim3(THREADS), 0, st, a);
+    if (a.headers) launch_overlapped(join_kernel<T, ROWS>, dim3(grid, ROWS), dim3(THREADS), 0, st, a);
+}
+
+template <typename T> int launch_paged(const PagedArgs &a, const Plan &p, cudaStream_t st) {
+    note_indexed_launch();
+    const int nv = 4;
+    bool vec = a.head_dim % nv == 0;
+    for (const void *x : {a.q, a.k, a.v}) vec = vec && reinterpret_cast<uintptr_t>(x) % (nv * sizeof(T)) == 0;
+    for (int64_t s : {a.sq_s, a.sq_h, a.sk_p, a.sk_h, a.sk_t, a.sv_p, a.sv_h, a.sv_t}) vec = vec && s % nv == 0;
+    if (a.head_dim > 128) {
+        if (p.rows == 1) launch_simple<T, 8, 1>(a, p.grid, vec, st);
+        else launch_simple<T, 8, 2>(a, p.grid, vec, st);
+    } else if (a.head_dim > 64) {
+        if (p.rows == 1) launch_simple<T, 4, 1>(a, p.grid, vec, st);
+        else launch_simple<T, 4, 4>(a, p.grid, vec, st);
+    } else {
+        if (p.rows == 1) launch_simple<T, 2, 1>(a, p.grid, vec, st);
+        else launch_simple<T, 2, 4>(a, p.grid, vec, st);
+    }
+    return check_launch("enc_paged_attention");
+}
+
+int check_paged(const enc_paged_cache *c, int64_t q_heads, int dtype, int variant, const char *me) {
+    if (!c) return fail(ENC_ERR_BAD_ARG, "%s: NULL cache", me);
+    if (!is_float_dtype(dtype)) return fail(ENC_ERR_BAD_ARG, "%s: dtype %d is not float16, bfloat16 or float32", me, dtype);
+    if (variant >= VARIANTS) return fail(ENC_ERR_BAD_ARG, "%s: variant %d out of range", me, variant);
+    const int bad = check_cache(*c, me);
+    if (bad) return bad;
+    if (c->head_dim > MAX_HEAD_DIM) return fail(ENC_ERR_UNSUPPORTED, "%s: head_dim %lld > %d", me, (long long)c->head_dim, MAX_HEAD_DIM);
+    if (q_heads < 1 || q_heads % c->kv_heads) return fail(ENC_ERR_BAD_ARG, "%s: %lld query heads over %lld kv heads", me, (long long)q_heads, (long long)c->kv_heads);
+    if (q_heads > 0xffff) return fail(ENC_ERR_UNSUPPORTED, "%s: more than 65535 query heads", me);
+    return 0;
+}
+
+}  // namespace
+
+unsigned int take_bad_index_paged_attention() { return take_bad_index_word(); }
+int paged_attention_variants() { return VARIANTS; }
+void paged_attention_variant_info(int, char *out, size_t n) {
+    snprintf(out, n, "CUDA cores, eight lanes per key, keys and values straight to registers");
+}
+
+}  // namespace enc
+
+extern "C" int64_t enc_paged_attention_work_bytes(const enc_paged_cache *cache, int64_t q_heads, int dtype, int variant) {
+    using namespace enc;
+    if (check_paged(cache, q_heads, dtype, variant, "enc_paged_attention_work_bytes")) return -1;
+    Plan p;
+    make_plan(*cache, q_heads, dtype, variant, p);
+    return p.work;
+}
+
+extern "C" int enc_paged_attention(const enc_paged_cache *cache, const void *q, void *o, float *lse, const int32_t *seq_lens,
+                                   int64_t q_heads, int64_t q_stride_seq, int64_t q_stride_head, int64_t o_stride_seq,
+                                   int64_t o_stride_head, float sm_scale, int64_t window, void *work, int64_t work_bytes,
+                                   int dtype, int variant, void *stream) {
+    ENC_PROLOGUE();
+    using namespace enc;
+    const char *me = "enc_paged_attention";
+    const int bad = check_paged(cache, q_heads, dtype, variant, me);
+    if (bad) return bad;
+    if (window < 0) return fail(ENC_ERR_BAD_ARG, "%s: negative window", me);
+    if (cache->num_seqs == 0) return ENC_OK;
+    if (!q || !o || !seq_lens) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
+    if ((!cache->k || !cache->v || !cache->block_table) && paged_capacity(*cache) > 0 && cache->num_pages > 0)
+        return fail(ENC_ERR_BAD_ARG, "%s: NULL cache tensor", me);
+    Plan p;
+    make_plan(*cache, q_heads, dtype, variant, p);
+    if (p.work > 0 && (!work || work_bytes < p.work || !aligned16(work)))
+        return fail(ENC_ERR_BAD_ARG, "%s: needs %lld bytes of 16-byte aligned workspace, got %lld", me, (long long)p.work, (long long)work_bytes);
+    PagedArgs a{};
+    a.q = q; a.k = cache->k; a.v = cache->v; a.o = o; a.lse = lse;
+    a.block_table = cache->block_table; a.seq_lens = seq_lens;
+    a.headers = p.work ? reinterpret_cast<int4 *>(work) : nullptr;
+    a.slots = p.work ? reinterpret_cast<float *>(reinterpret_cast<char *>(work) + (int64_t)p.grid * 16) : nullptr;
+    a.sq_s = q_stride_seq; a.sq_h = q_stride_head; a.so_s = o_stride_seq; a.so_h = o_stride_head;
+    a.sk_p = cache->k_stride_page; a.sk_h = cache->k_stride_head; a.sk_t = cache->k_stride_token;
+    a.sv_p = cache->v_stride_page; a.sv_h = cache->v_stride_head; a.sv_t = cache->v_stride_token;
+    a.s_table = cache->stride_table;
+    a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.capacity = paged_capacity(*cache); a.window = window;
+    a.q_heads = (int)q_heads; a.head_dim = (int)cache->head_dim; a.group = (int)(q_heads / cache->kv_heads);
+    a.row_groups = p.row_groups; a.units = (int)cache->kv_heads * p.row_groups;
+    a.min_run = 1;
+    a.scale = sm_scale * LOG2E;
+    a.page_size = FastDiv((uint32_t)cache->page_size);
+    cudaStream_t st = as_stream(stream);
+    switch (dtype) {
+        case ENC_F16: return launch_paged<__half>(a, p, st);
+        case ENC_BF16: return launch_paged<__nv_bfloat16>(a, p, st);
+        default: return launch_paged<float>(a, p, st);
+    }
+}

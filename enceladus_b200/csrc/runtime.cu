@@ -1,5 +1,6 @@
 // Host-side runtime of the kernel library: status strings, device properties, the device error
 // word that bounded device-side waits raise, variant tables and synchronisation.
+#include <atomic>
 #include <mutex>
 
 #include "sm100.cuh"
@@ -20,6 +21,15 @@ int attention_variants();
 void attention_variant_info(int v, char *out, size_t n);
 int int_matmul_variants();
 void int_matmul_variant_info(int v, char *out, size_t n);
+int append_variants();
+void append_variant_info(int v, char *out, size_t n);
+unsigned int take_bad_index_append();
+int paged_attention_variants();
+void paged_attention_variant_info(int v, char *out, size_t n);
+unsigned int take_bad_index_paged_attention();
+int logits_variants();
+void logits_variant_info(int v, char *out, size_t n);
+unsigned int take_bad_index_logits();
 
 namespace {
 thread_local char g_error[1024] = "";
@@ -28,6 +38,7 @@ constexpr int MAX_DEVICES = 64;
 std::mutex g_mu;
 DeviceProps g_props[MAX_DEVICES];
 unsigned int *g_error_word[MAX_DEVICES];
+std::atomic<bool> g_indexed[MAX_DEVICES];  // a kernel that reads index arrays has been launched on this device
 }  // namespace
 
 int fail(int status, const char *fmt, ...) {
@@ -50,6 +61,12 @@ int check_launch(const char *what) {
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) return ENC_OK;
     return fail(ENC_ERR_LAUNCH, "%s: CUDA error %d (%s)", what, (int)e, cudaGetErrorString(e));
+}
+
+void note_indexed_launch() {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < MAX_DEVICES) g_indexed[dev].store(true, std::memory_order_relaxed);
 }
 
 const DeviceProps &device_props() {
@@ -183,6 +200,9 @@ extern "C" int enc_num_variants(int kernel) {
         case ENC_K_MATMUL: return enc::matmul_variants();
         case ENC_K_ATTENTION: return enc::attention_variants();
         case ENC_K_MATMUL_INT: return enc::int_matmul_variants();
+        case ENC_K_APPEND_KV: return enc::append_variants();
+        case ENC_K_PAGED_ATTENTION: return enc::paged_attention_variants();
+        case ENC_K_LOGITS: return enc::logits_variants();
         case ENC_K_ADD: return 1;
         default: return 0;
     }
@@ -200,6 +220,9 @@ extern "C" int enc_variant_info(int kernel, int variant, char *out, size_t n) {
         case ENC_K_MATMUL: enc::matmul_variant_info(variant, out, n); break;
         case ENC_K_ATTENTION: enc::attention_variant_info(variant, out, n); break;
         case ENC_K_MATMUL_INT: enc::int_matmul_variant_info(variant, out, n); break;
+        case ENC_K_APPEND_KV: enc::append_variant_info(variant, out, n); break;
+        case ENC_K_PAGED_ATTENTION: enc::paged_attention_variant_info(variant, out, n); break;
+        case ENC_K_LOGITS: enc::logits_variant_info(variant, out, n); break;
         default: snprintf(out, n, "cta_threads=256 grid-stride"); break;
     }
     return ENC_OK;
@@ -227,6 +250,12 @@ extern "C" int enc_synchronize(void *stream) {
             cudaMemset(w, 0, sizeof(host));
             return enc::fail(ENC_ERR_DEVICE_WAIT, "a device-side wait ran out of its iteration limit (status word %u); results of the launches since the last synchronisation are invalid", host);
         }
+    }
+    if (dev >= 0 && dev < enc::MAX_DEVICES && enc::g_indexed[dev].load(std::memory_order_relaxed)) {
+        const unsigned append = enc::take_bad_index_append(), attend = enc::take_bad_index_paged_attention(), logits = enc::take_bad_index_logits();
+        if (append | attend | logits)
+            return enc::fail(ENC_ERR_BAD_INDEX, "an index array held a value out of range (%s%s%s); what it named was skipped and results of the launches since the last synchronisation are incomplete",
+                             append ? "enc_append_kv " : "", attend ? "enc_paged_attention " : "", logits ? "enc_penalize_logits " : "");
     }
     return ENC_OK;
 }

@@ -279,3 +279,214 @@ def cumsum(x, reverse: bool = False):
     cumsum_kernel[(enceladus.cdiv(m, block_m),)](out, x, m, n, si, so, REVERSE=reverse, BLOCK_M=block_m,
                                                  BLOCK_N=block_n)
     return out
+
+
+# ---- the decoding step: paged key-value cache, attention of one new token, logits -----------------------
+def _no_overlap(x, what: str) -> None:
+    """Refuses an output whose elements share memory (an expanded view), where writes would meet."""
+    if any(n > 1 and s == 0 for n, s in zip(x.shape, enceladus.element_strides(x))):
+        raise ValueError(f"{what} is written, so its elements can't share memory (a stride is 0)")
+
+
+def _check_cache(k_cache, v_cache, block_table):
+    if len(k_cache.shape) != 4 or tuple(k_cache.shape) != tuple(v_cache.shape):
+        raise ValueError("k_cache and v_cache must both have shape (pages, kv_heads, page_size, head_dim), but got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if len(block_table.shape) != 2:
+        raise ValueError(f"block_table must have shape (sequences, pages per sequence), not {tuple(block_table.shape)}")
+    ks, vs = enceladus.element_strides(k_cache), enceladus.element_strides(v_cache)
+    ts = enceladus.element_strides(block_table)
+    for x, st, what in ((k_cache, ks, "k_cache"), (v_cache, vs, "v_cache"), (block_table, ts, "block_table")):
+        if x.shape[-1] > 1 and st[-1] != 1 and 0 not in x.shape:
+            raise ValueError(f"the last dimension of {what} must be contiguous")
+    return ks, vs, ts[0]
+
+
+def _check_heads(x, what: str, rows: int, head_dim: int, heads: int | None = None):
+    """Strides of a (rows, heads, head_dim) array with contiguous heads."""
+    if len(x.shape) != 3 or x.shape[0] != rows or x.shape[2] != head_dim or (heads is not None and x.shape[1] != heads):
+        raise ValueError(f"{what} must have shape ({rows}, {'heads' if heads is None else heads}, {head_dim}), not {tuple(x.shape)}")
+    st = enceladus.element_strides(x)
+    if head_dim > 1 and st[2] != 1 and 0 not in x.shape:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return st
+
+
+def _check_row(x, what: str, n: int) -> None:
+    if len(x.shape) != 1 or x.shape[0] != n or (n > 1 and enceladus.element_strides(x)[0] != 1):
+        raise ValueError(f"{what} must be contiguous with shape ({n},), not {tuple(x.shape)}")
+
+
+@enceladus.jit
+def append_kv_kernel(k_ptr, v_ptr, q_ptr, q_out_ptr, k_cache_ptr, v_cache_ptr, block_table_ptr, seq_ids_ptr, positions_ptr, cos_ptr,
+                     sin_ptr, n_seqs, table_width, stride_table, n_pages, n_positions, stride_k_token, stride_k_head, stride_v_token,
+                     stride_v_head, stride_q_token, stride_q_head, stride_o_token, stride_o_head, stride_cos, stride_kp, stride_kh,
+                     stride_kt, stride_vp, stride_vh, stride_vt, Q_HEADS: tl.constexpr, KV_HEADS: tl.constexpr,
+                     HEAD_DIM: tl.constexpr, ROT_DIM: tl.constexpr, PAGE_SIZE: tl.constexpr, INTERLEAVED: tl.constexpr):
+    """One token per program: k and v go to row positions[t] % PAGE_SIZE of page block_table[seq_ids[t], positions[t] // PAGE_SIZE];
+    the first ROT_DIM elements of every k and q head turn in pairs by cos / sin of the token's position, in float32."""
+
+
+def append_kv(k, v, k_cache, v_cache, block_table, seq_ids, positions, cos=None, sin=None, q=None, q_out=None,
+              interleaved: bool = False):
+    """Appends one key and value per token to a paged cache, in place, and returns the rotated `q` (None without `q`).
+
+    `k` and `v` have shape (tokens, kv_heads, head_dim), `q` (tokens, q_heads, head_dim); slices of one fused
+    projection will do, only the heads' elements must be contiguous. The caches have shape (pages, kv_heads,
+    page_size, head_dim) with any strides: a cache laid out token by token is passed as `cache.transpose(1, 2)`.
+    Token `t` is token `positions[t]` of sequence `seq_ids[t]`, whose pages `block_table[seq_ids[t]]` lists; a
+    negative `seq_ids[t]` marks padding, for which nothing is written. All index arrays are int32. Prompts and
+    single tokens mix freely, but no two tokens of a call may be the same token of a sequence, nor two sequences
+    write to one shared page.
+
+    `cos` and `sin`, float32 of shape (positions, rot_dim / 2), turn the first `rot_dim` elements of each query and
+    key head: elements `(i, i + rot_dim / 2)` together, or `(2i, 2i + 1)` when `interleaved`. Without them nothing
+    turns. `q_out` may be `q`. A sequence, position or page out of range is skipped, and `synchronize()` raises
+    `CudaError`.
+    """
+    ks, vs, st = _check_cache(k_cache, v_cache, block_table)
+    pages, kv_heads, page_size, d = k_cache.shape
+    tokens = k.shape[0]
+    k_st, v_st = _check_heads(k, "k", tokens, d, kv_heads), _check_heads(v, "v", tokens, d, kv_heads)
+    _check_row(seq_ids, "seq_ids", tokens)
+    _check_row(positions, "positions", tokens)
+    _no_overlap(k_cache, "k_cache")
+    _no_overlap(v_cache, "v_cache")
+    q_st = o_st = (0, 0, 0)
+    q_heads = 0
+    if q is not None:
+        q_st, q_heads = _check_heads(q, "q", tokens, d), q.shape[1]
+        if q_out is None:
+            q_out = enceladus.new_empty(q)
+        o_st = _check_heads(q_out, "q_out", tokens, d, q_heads)
+        _no_overlap(q_out, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    n_positions = rot_dim = cos_st = 0
+    if cos is not None:
+        if len(cos.shape) != 2 or tuple(cos.shape) != tuple(sin.shape) or 2 * cos.shape[1] > d:
+            raise ValueError(f"cos and sin must both have shape (positions, rot_dim / 2) with rot_dim <= {d}, but got "
+                             f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+        c, s = enceladus.element_strides(cos), enceladus.element_strides(sin)
+        if c != s or (cos.shape[1] > 1 and c[1] != 1):
+            raise ValueError("cos and sin must have the same strides and contiguous rows")
+        n_positions, rot_dim, cos_st = cos.shape[0], 2 * cos.shape[1], c[0]
+        if not rot_dim:
+            cos = sin = None
+    append_kv_kernel[(tokens,)](k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, block_table.shape[0],
+                                block_table.shape[1], st, pages, n_positions, k_st[0], k_st[1], v_st[0], v_st[1], q_st[0], q_st[1],
+                                o_st[0], o_st[1], cos_st, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,
+                                KV_HEADS=kv_heads, HEAD_DIM=d, ROT_DIM=rot_dim, PAGE_SIZE=page_size, INTERLEAVED=interleaved)
+    return q_out
+
+
+@enceladus.jit
+def paged_attention_kernel(q_ptr, k_cache_ptr, v_cache_ptr, o_ptr, lse_ptr, block_table_ptr, seq_lens_ptr, sm_scale, window, table_width,
+                           stride_table, n_pages, stride_qs, stride_qh, stride_os, stride_oh, stride_kp, stride_kh, stride_kt,
+                           stride_vp, stride_vh, stride_vt, Q_HEADS: tl.constexpr, KV_HEADS: tl.constexpr, HEAD_DIM: tl.constexpr,
+                           PAGE_SIZE: tl.constexpr):
+    """softmax(q k^T * sm_scale) v of one query token per sequence over the sequence's keys in a paged cache: base-2 online
+    softmax in float32, the probabilities not rounded; lse = ln2 * (m + log2 l)."""
+
+
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale: float | None = None, window: int = 0, o=None,
+                    return_lse: bool = False):
+    """Returns `softmax(q @ k^T * sm_scale) @ v` for one new token per sequence over a paged cache, in the input dtype.
+
+    `q` has shape (sequences, q_heads, head_dim), head_dim at most 256; the caches and `block_table` are those of
+    `append_kv`, with `q_heads` a multiple of the cache's heads. Sequence `s` looks at its first `seq_lens[s]` (int32)
+    tokens, or the last `window` of them when `window` is positive. A sequence of length zero gives zeros, and so does
+    a row whose weights are all zero. What the cache holds past a sequence's length doesn't matter.
+
+    With `return_lse=True`, also returns the float32 log-sum-exp of the scaled scores, shape (sequences, q_heads):
+    -inf for a row without keys. A length or page out of range is cut or skipped, and `synchronize()` raises `CudaError`.
+    """
+    ks, vs, st = _check_cache(k_cache, v_cache, block_table)
+    pages, kv_heads, page_size, d = k_cache.shape
+    seqs = q.shape[0]
+    q_st = _check_heads(q, "q", seqs, d)
+    q_heads = q.shape[1]
+    if kv_heads == 0 or q_heads == 0 or q_heads % kv_heads:
+        raise ValueError(f"the query heads must be a multiple of the cache's heads, but got {q_heads} and {kv_heads}")
+    if not 1 <= d <= 256:
+        raise ValueError(f"head_dim must be from 1 to 256, not {d}")
+    if block_table.shape[0] != seqs:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows, but q has {seqs}")
+    _check_row(seq_lens, "seq_lens", seqs)
+    if window < 0:
+        raise ValueError(f"window can't be negative, but got {window}")
+    if o is None:
+        o = enceladus.new_empty(q)
+    else:
+        _no_overlap(o, "o")
+    o_st = _check_heads(o, "o", seqs, d, q_heads)
+    scale = 1.0 / math.sqrt(d) if sm_scale is None else sm_scale
+    lse = enceladus.new_empty(q, (seqs, q_heads), np.float32) if return_lse else None
+    paged_attention_kernel[(seqs,)](q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, block_table.shape[1], st, pages,
+                                    q_st[0], q_st[1], o_st[0], o_st[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,
+                                    KV_HEADS=kv_heads, HEAD_DIM=d, PAGE_SIZE=page_size)
+    return (o, lse) if return_lse else o
+
+
+@enceladus.jit
+def penalize_logits_kernel(logits_ptr, out_ptr, tokens_ptr, lens_ptr, prompt_lens_ptr, repetition_ptr, frequency_ptr, presence_ptr,
+                           bias_ids_ptr, bias_values_ptr, mask_ptr, vocab, stride_in, stride_out, history, stride_tokens, n_biases,
+                           stride_bias, stride_mask):
+    """One row per program: penalties for the tokens of the row's history, biases, then -inf where the mask bit is clear."""
+
+
+def penalize_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=None, frequency=None, presence=None,
+                    bias_ids=None, bias_values=None, mask=None, out=None):
+    """Returns `logits` (rows, vocab) with penalties, biases and a grammar mask applied, in the input dtype.
+
+    The first `lens[r]` of `tokens[r]` are row `r`'s history, the first `prompt_lens[r]` of them its prompt (int32).
+    In this order, in float32: a logit whose token is in the history is divided by `repetition[r]` if positive and
+    multiplied by it otherwise; one whose token was generated (is behind the prompt) `n > 0` times loses
+    `frequency[r] * n + presence[r]`; `bias_values[r, i]` (float32) is added to token `bias_ids[r, i]` (int32; -1: an
+    unused place; a token that occurs twice gets both); a token whose bit in `mask` is clear becomes -inf, whatever
+    it was: bit `t % 32` of word `mask[r, t // 32]` (int32) is set for a token that is allowed. A row that allows
+    nothing is -inf throughout.
+
+    The history's arrays come together, the biases' too, and each part can be left out. `out` may be `logits`.
+    A token, bias id or length out of range is ignored or cut, and `synchronize()` raises `CudaError`.
+    """
+    if len(logits.shape) != 2:
+        raise ValueError(f"logits must have shape (rows, vocab), not {tuple(logits.shape)}")
+    m, n = logits.shape
+
+    def rows_of(x, what, cols=None):
+        if len(x.shape) != 2 or x.shape[0] != m or (cols is not None and x.shape[1] != cols):
+            raise ValueError(f"{what} must have shape ({m}, {'...' if cols is None else cols}), not {tuple(x.shape)}")
+        st = enceladus.element_strides(x)
+        if x.shape[1] > 1 and st[1] != 1:
+            raise ValueError(f"the rows of {what} must be contiguous")
+        return st[0]
+
+    si = rows_of(logits, "logits")
+    past = (tokens, lens, prompt_lens, repetition, frequency, presence)
+    if any(x is None for x in past) and any(x is not None for x in past):
+        raise ValueError("tokens, lens, prompt_lens, repetition, frequency and presence go together")
+    history = stride_tokens = n_biases = stride_bias = stride_mask = 0
+    if tokens is not None:
+        history, stride_tokens = tokens.shape[-1], rows_of(tokens, "tokens")
+        for x, what in zip(past[1:], ("lens", "prompt_lens", "repetition", "frequency", "presence")):
+            _check_row(x, what, m)
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    if bias_ids is not None:
+        n_biases, stride_bias = bias_ids.shape[-1], rows_of(bias_ids, "bias_ids")
+        if rows_of(bias_values, "bias_values", n_biases) != stride_bias and m > 1:
+            raise ValueError("bias_ids and bias_values must have the same strides")
+    if mask is not None:
+        stride_mask = rows_of(mask, "mask", enceladus.cdiv(n, 32))
+        if m == 1:  # the stride of a single row means nothing
+            stride_mask = mask.shape[1]
+    if out is None:
+        out = enceladus.new_empty(logits)
+    else:
+        _no_overlap(out, "out")
+    penalize_logits_kernel[(m,)](logits, out, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, mask,
+                                 n, si, rows_of(out, "out", n), history, stride_tokens, n_biases, stride_bias, stride_mask)
+    return out

@@ -271,6 +271,8 @@ class JITFunction:
             lines.append(f"  grid {resolve_grid(grid, {k: (v.value if isinstance(v, tl.constexpr) else v) for k, v in bound.items()})}")
         for name in ad.array_list:
             a = bound[name]
+            if a is None:
+                continue  # an optional array that this launch goes without
             role = "out" if name in ad.outputs else "in"
             lines.append(f"  {role:3s} {name}: {getattr(a, 'dtype', type(a).__name__)} {tuple(getattr(a, 'shape', ()))}")
         consts = {n: bound[n] for n in self._constexpr_names}
@@ -306,7 +308,8 @@ class CompiledKernel:
 _ENTRY_POINTS = {N.K_SOFTMAX: "enc_softmax", N.K_LAYERNORM: "enc_layernorm", N.K_RMSNORM: "enc_rmsnorm",
                  N.K_GELU: "enc_gelu", N.K_MATMUL: "enc_matmul", N.K_ATTENTION: "enc_attention_fwd",
                  N.K_HISTOGRAM: "enc_histogram", N.K_CUMSUM: "enc_cumsum", N.K_ADD: "enc_add",
-                 N.K_MATMUL_INT: "enc_matmul_int"}
+                 N.K_MATMUL_INT: "enc_matmul_int", N.K_APPEND_KV: "enc_append_kv",
+                 N.K_PAGED_ATTENTION: "enc_paged_attention", N.K_LOGITS: "enc_penalize_logits"}
 
 
 def launch(ad, bound: dict[str, Any], grid: tuple[int, int, int], variant: int, jf: JITFunction | None) -> None:
@@ -328,7 +331,7 @@ def launch(ad, bound: dict[str, Any], grid: tuple[int, int, int], variant: int, 
                                  "all array arguments of one launch must be on the same device")
         elif isinstance(v, np.ndarray):
             host_names = [name] if host_names is None else [*host_names, name]
-        else:
+        elif v is not None or name not in ad.optional:
             raise TypeError(f"argument `{name}` must be a NumPy array or a torch CUDA tensor, not "
                             f"{type(v).__name__}")
     torch = interop._torch()

@@ -51,6 +51,8 @@ class Adapter:
     extents: Callable[[dict[str, Any], tuple[int, int, int]], dict[str, int]] | None = field(repr=False, default=None)
     # how to cut a launch into independent pieces, or None when the kernel has no such cut
     split: Callable[[dict[str, Any], tuple[int, int, int]], Split | None] | None = field(repr=False, default=None)
+    # arrays that a launch may go without (None in their place)
+    optional: frozenset[str] = frozenset()
 
     def __post_init__(self) -> None:
         self.array_list = tuple(p for p in self.params if p in self.arrays)
@@ -62,10 +64,11 @@ class Adapter:
 _REGISTRY: dict[str, Adapter] = {}
 
 
-def register(name: str, params: str, arrays: str, outputs: str, kernel_id: int, extents=None, split=None):
+def register(name: str, params: str, arrays: str, outputs: str, kernel_id: int, extents=None, split=None,
+             optional: str = ""):
     def deco(fn):
         _REGISTRY[name] = Adapter(name, tuple(params.split()), frozenset(arrays.split()),
-                                  frozenset(outputs.split()), kernel_id, fn, extents, split)
+                                  frozenset(outputs.split()), kernel_id, fn, extents, split, frozenset(optional.split()))
         return fn
 
     return deco
@@ -339,3 +342,91 @@ def _attention_lse(a, grid, variant, stream):
            float(a["sm_scale"]), int(bool(a["CAUSAL"])), dt, variant, stream)
 
 
+
+
+# ---- the decoding step: paged cache, attention of one new token, logits -----------------------------
+def _opt(t: Any) -> int | None:
+    return None if t is None else int(t.data_ptr())
+
+
+def _need(a: dict[str, Any], code: int, *names: str) -> None:
+    for n in names:
+        if a[n] is not None and _code(a[n]) != code:
+            raise TypeError(f"argument `{n}` must be {'int32' if code == N.I32 else 'float32'}, not {interop.element_dtype(a[n])}")
+
+
+_CACHE_STRIDES = "stride_kp stride_kh stride_kt stride_vp stride_vh stride_vt"
+
+
+def _paged_cache(a: dict[str, Any], seqs: int) -> N.PagedCache:
+    return N.PagedCache(_ptr(a["k_cache_ptr"]), _ptr(a["v_cache_ptr"]), _ptr(a["block_table_ptr"]), int(a["n_pages"]), int(a["PAGE_SIZE"]),
+                        int(a["KV_HEADS"]), int(a["HEAD_DIM"]), seqs, int(a["table_width"]), int(a["stride_table"]), int(a["stride_kp"]),
+                        int(a["stride_kh"]), int(a["stride_kt"]), int(a["stride_vp"]), int(a["stride_vh"]), int(a["stride_vt"]))
+
+
+# grid[0] = tokens.  The caches are written in place, so a NumPy cache is copied in and back whole.
+@register("append_kv_kernel",
+          "k_ptr v_ptr q_ptr q_out_ptr k_cache_ptr v_cache_ptr block_table_ptr seq_ids_ptr positions_ptr cos_ptr sin_ptr "
+          "n_seqs table_width stride_table n_pages n_positions stride_k_token stride_k_head stride_v_token stride_v_head "
+          "stride_q_token stride_q_head stride_o_token stride_o_head stride_cos " + _CACHE_STRIDES +
+          " Q_HEADS KV_HEADS HEAD_DIM ROT_DIM PAGE_SIZE INTERLEAVED",
+          "k_ptr v_ptr q_ptr q_out_ptr k_cache_ptr v_cache_ptr block_table_ptr seq_ids_ptr positions_ptr cos_ptr sin_ptr",
+          "q_out_ptr k_cache_ptr v_cache_ptr", N.K_APPEND_KV, optional="q_ptr q_out_ptr cos_ptr sin_ptr")
+def _append_kv(a, grid, variant, stream):
+    names = ("k_ptr", "v_ptr", "k_cache_ptr", "v_cache_ptr")
+    if (a["q_ptr"] is None) != (a["q_out_ptr"] is None):
+        raise TypeError("append_kv_kernel: `q_ptr` and `q_out_ptr` go together")
+    if a["q_ptr"] is not None:
+        names += ("q_ptr", "q_out_ptr")
+    dt = _same_dtype(a, *names)
+    _need(a, N.I32, "block_table_ptr", "seq_ids_ptr", "positions_ptr")
+    _need(a, N.F32, "cos_ptr", "sin_ptr")
+    N.call("enc_append_kv", _paged_cache(a, int(a["n_seqs"])), _ptr(a["k_ptr"]), _ptr(a["v_ptr"]), _opt(a["q_ptr"]), _opt(a["q_out_ptr"]),
+           _opt(a["cos_ptr"]), _opt(a["sin_ptr"]), _ptr(a["seq_ids_ptr"]), _ptr(a["positions_ptr"]), grid[0], int(a["Q_HEADS"]),
+           int(a["ROT_DIM"]), int(bool(a["INTERLEAVED"])), int(a["n_positions"]), int(a["stride_k_token"]), int(a["stride_k_head"]),
+           int(a["stride_v_token"]), int(a["stride_v_head"]), int(a["stride_q_token"]), int(a["stride_q_head"]),
+           int(a["stride_o_token"]), int(a["stride_o_head"]), int(a["stride_cos"]), dt, variant, stream)
+
+
+# grid[0] = sequences.  The buffer for split rows comes from torch's caching allocator on the launch's stream: nothing is
+# shared with other launches, and a captured launch keeps the one it was captured with.
+@register("paged_attention_kernel",
+          "q_ptr k_cache_ptr v_cache_ptr o_ptr lse_ptr block_table_ptr seq_lens_ptr sm_scale window table_width stride_table n_pages "
+          "stride_qs stride_qh stride_os stride_oh " + _CACHE_STRIDES + " Q_HEADS KV_HEADS HEAD_DIM PAGE_SIZE",
+          "q_ptr k_cache_ptr v_cache_ptr o_ptr lse_ptr block_table_ptr seq_lens_ptr", "o_ptr lse_ptr", N.K_PAGED_ATTENTION,
+          extents=lambda a, g: {"lse_ptr": g[0] * int(a["Q_HEADS"]), **({"o_ptr": g[0] * int(a["Q_HEADS"]) * int(a["HEAD_DIM"])} if int(a["stride_oh"]) == int(a["HEAD_DIM"]) and int(a["stride_os"]) == int(a["Q_HEADS"]) * int(a["HEAD_DIM"]) else {})},
+          optional="lse_ptr")
+def _paged_attention(a, grid, variant, stream):
+    dt = _same_dtype(a, "q_ptr", "k_cache_ptr", "v_cache_ptr", "o_ptr")
+    _need(a, N.I32, "block_table_ptr", "seq_lens_ptr")
+    _need(a, N.F32, "lse_ptr")
+    cache, q_heads = _paged_cache(a, grid[0]), int(a["Q_HEADS"])
+    nbytes = N.load().enc_paged_attention_work_bytes(cache, q_heads, dt, variant)
+    if nbytes < 0:
+        N.check(N.ERR_BAD_ARG)
+    work = None
+    if nbytes:
+        torch = interop._torch()
+        work = torch.empty(nbytes, dtype=torch.uint8, device=a["q_ptr"].device)
+    N.call("enc_paged_attention", cache, _ptr(a["q_ptr"]), _ptr(a["o_ptr"]), _opt(a["lse_ptr"]), _ptr(a["seq_lens_ptr"]), q_heads,
+           int(a["stride_qs"]), int(a["stride_qh"]), int(a["stride_os"]), int(a["stride_oh"]), float(a["sm_scale"]), int(a["window"]),
+           _opt(work), nbytes, dt, variant, stream)
+
+
+# grid[0] = rows
+@register("penalize_logits_kernel",
+          "logits_ptr out_ptr tokens_ptr lens_ptr prompt_lens_ptr repetition_ptr frequency_ptr presence_ptr bias_ids_ptr bias_values_ptr "
+          "mask_ptr vocab stride_in stride_out history stride_tokens n_biases stride_bias stride_mask",
+          "logits_ptr out_ptr tokens_ptr lens_ptr prompt_lens_ptr repetition_ptr frequency_ptr presence_ptr bias_ids_ptr bias_values_ptr "
+          "mask_ptr", "out_ptr", N.K_LOGITS,
+          extents=lambda a, g: {"out_ptr": g[0] * int(a["vocab"])} if int(a["stride_out"]) == int(a["vocab"]) else {},
+          optional="tokens_ptr lens_ptr prompt_lens_ptr repetition_ptr frequency_ptr presence_ptr bias_ids_ptr bias_values_ptr mask_ptr")
+def _penalize_logits(a, grid, variant, stream):
+    dt = _same_dtype(a, "logits_ptr", "out_ptr")
+    _need(a, N.I32, "tokens_ptr", "lens_ptr", "prompt_lens_ptr", "bias_ids_ptr", "mask_ptr")
+    _need(a, N.F32, "repetition_ptr", "frequency_ptr", "presence_ptr", "bias_values_ptr")
+    N.call("enc_penalize_logits", _ptr(a["logits_ptr"]), _ptr(a["out_ptr"]), grid[0], int(a["vocab"]), int(a["stride_in"]),
+           int(a["stride_out"]), _opt(a["tokens_ptr"]), int(a["history"]), int(a["stride_tokens"]), _opt(a["lens_ptr"]),
+           _opt(a["prompt_lens_ptr"]), _opt(a["repetition_ptr"]), _opt(a["frequency_ptr"]), _opt(a["presence_ptr"]),
+           _opt(a["bias_ids_ptr"]), _opt(a["bias_values_ptr"]), int(a["n_biases"]), int(a["stride_bias"]), _opt(a["mask_ptr"]),
+           int(a["stride_mask"]), dt, variant, stream)

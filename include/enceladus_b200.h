@@ -39,7 +39,8 @@ typedef enum {
     ENC_ERR_UNSUPPORTED = 2,  /* valid request this build has no kernel for                    */
     ENC_ERR_LAUNCH = 3,       /* CUDA reported an error at launch / in an earlier async launch */
     ENC_ERR_DEVICE_WAIT = 4,  /* a bounded device-side wait ran out (reported at sync)         */
-    ENC_ERR_NO_MEMORY = 5     /* scratch allocation failed                                     */
+    ENC_ERR_NO_MEMORY = 5,    /* scratch allocation failed                                     */
+    ENC_ERR_BAD_INDEX = 6     /* an index array held a value out of range (reported at sync)   */
 } enc_status;
 
 typedef enum {
@@ -64,7 +65,10 @@ typedef enum {
     ENC_K_CUMSUM = 7,
     ENC_K_ADD = 8,
     ENC_K_MATMUL_INT = 9,
-    ENC_K_COUNT = 10
+    ENC_K_APPEND_KV = 10,
+    ENC_K_PAGED_ATTENTION = 11,
+    ENC_K_LOGITS = 12,
+    ENC_K_COUNT = 13
 } enc_kernel;
 
 #define ENC_VARIANT_AUTO (-1)
@@ -223,6 +227,76 @@ int enc_matmul_int(const void *a, const void *b, void *c, int64_t M, int64_t N, 
 int enc_attention_fwd(const void *q, const void *k, const void *v, void *o, float *lse, int64_t bh,
                       int64_t seq, int64_t head_dim, int64_t stride_h, int64_t stride_m,
                       float sm_scale, int causal, int dtype, int variant, void *stream);
+
+/* ---- decoding step -------------------------------------------------------------------------- */
+
+/* A paged key-value cache.  k and v are pools of num_pages pages; a page holds page_size tokens of kv_heads heads
+ * of head_dim elements.  Any layout with contiguous head elements is described by its strides (page-head-token-dim
+ * and page-token-head-dim alike), k and v each with their own.  block_table[s * stride_table + i] is the page that holds
+ * tokens i*page_size .. (i+1)*page_size-1 of sequence s.  Several sequences may name the same page (a shared prefix). */
+typedef struct {
+    void *k, *v;
+    const int32_t *block_table; /* [num_seqs, table_width]                        */
+    int64_t num_pages, page_size, kv_heads, head_dim;
+    int64_t num_seqs, table_width, stride_table;
+    int64_t k_stride_page, k_stride_head, k_stride_token;
+    int64_t v_stride_page, v_stride_head, v_stride_token;
+} enc_paged_cache;
+
+/* Appends one key and one value per token to the cache and rotates queries and keys by their positions on the way.
+ * Token t belongs to sequence seq_ids[t] and has position positions[t] in it; seq_ids[t] < 0 marks padding: nothing is
+ * read or written for that token.  Of every query and key head the first rot_dim elements turn in pairs,
+ *   a' = a*cos - b*sin,  b' = b*cos + a*sin,   (a, b) = elements (i, i + rot_dim/2), or (2i, 2i+1) when `interleaved`,
+ * in float32 with one rounding, by cos / sin [num_positions, rot_dim/2] (float32, rows stride_cos apart) at the token's
+ * position; the other elements and the values are copied.  q and q_out may be NULL (no queries) or the same tensor;
+ * rot_dim 0 (cos and sin then unused) appends without rotation.
+ * k, v: [tokens, kv_heads, head_dim], q, q_out: [tokens, q_heads, head_dim], strides per token and head, elements of a
+ * head contiguous.  All share `dtype` (ENC_F32 | ENC_F16 | ENC_BF16) with the cache.
+ * A token whose sequence, position or page is out of range is skipped and enc_synchronize returns ENC_ERR_BAD_INDEX.
+ * Two tokens of one call must not name the same place in the cache: which of them stays there is not defined.
+ * No counterpart in the reference, whose attention (examples/08_flash_attention.py:30-103) has no cache. */
+int enc_append_kv(const enc_paged_cache *cache, const void *k, const void *v, const void *q, void *q_out,
+                  const float *cos, const float *sin, const int32_t *seq_ids, const int32_t *positions,
+                  int64_t tokens, int64_t q_heads, int64_t rot_dim, int interleaved, int64_t num_positions,
+                  int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
+                  int64_t q_stride_token, int64_t q_stride_head, int64_t o_stride_token, int64_t o_stride_head,
+                  int64_t stride_cos, int dtype, int variant, void *stream);
+
+/* Attention of one new token per sequence over the cache: for every sequence s < cache->num_seqs and query head h,
+ * o[s, h] = softmax(q[s, h] . K^T * sm_scale) V over the first seq_lens[s] tokens of the sequence (the last `window` of
+ * them when window > 0), with head h reading kv head h / (q_heads / kv_heads).  Statistics and sums in float32.  A row
+ * without keys (length zero), or whose weights sum to zero, is zero with lse -inf.  lse: float32 [num_seqs, q_heads] or
+ * NULL.  Cache contents past a sequence's length are never used.
+ * q, o: [num_seqs, q_heads, head_dim] with strides per sequence and head; all of `dtype`; head_dim <= 256.
+ * The keys of all sequences and heads are dealt out evenly over the GPU, whatever their lengths: the schedule is computed
+ * on the device from seq_lens, so a captured launch follows the lengths it finds.  Pieces that do not finish a row go
+ * through `work`, a buffer of at least enc_paged_attention_work_bytes() bytes, 16-byte aligned, whose contents need
+ * no preparation and mean nothing afterwards; launches that may overlap need buffers of their own.
+ * A length or page out of range is cut or skipped and enc_synchronize returns ENC_ERR_BAD_INDEX.
+ * Counterpart in the reference for a whole sequence without a cache: examples/08_flash_attention.py:30-103 */
+int enc_paged_attention(const enc_paged_cache *cache, const void *q, void *o, float *lse, const int32_t *seq_lens,
+                        int64_t q_heads, int64_t q_stride_seq, int64_t q_stride_head, int64_t o_stride_seq,
+                        int64_t o_stride_head, float sm_scale, int64_t window, void *work, int64_t work_bytes,
+                        int dtype, int variant, void *stream);
+/* Bytes of `work` for enc_paged_attention with these arguments on the current device (0: none is needed); -1 on a bad argument. */
+int64_t enc_paged_attention_work_bytes(const enc_paged_cache *cache, int64_t q_heads, int dtype, int variant);
+
+/* Penalties, biases and grammar masks on logits [rows, vocab], one pass, float32 arithmetic, output in `dtype`:
+ *   x = logits[r, t]
+ *   t among tokens[r, :lens[r]]                         : x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   t n > 0 times in tokens[r, prompt_lens[r]:lens[r]]  : x = x - (frequency[r] * n + presence[r])
+ *   x = x + (sum of bias_values[r, i] with bias_ids[r, i] == t, in order of i)
+ *   bit t % 32 of mask[r, t / 32] clear                 : x = -inf
+ * tokens (int32 [rows, .], rows stride_tokens apart, `history` columns), lens, prompt_lens, repetition, frequency and
+ * presence come together or are all NULL; bias_ids / bias_values [rows, num_biases] (an id of -1 is an unused place) and
+ * mask [rows, stride_mask words] each may be NULL.  out may be logits itself.  Masked logits are -inf whatever they were.
+ * A token, id or length out of range is ignored or cut and enc_synchronize returns ENC_ERR_BAD_INDEX.
+ * No counterpart in the reference; the rows continue in softmax_kernel, examples/02_softmax.py:15-38 */
+int enc_penalize_logits(const void *logits, void *out, int64_t rows, int64_t vocab, int64_t stride_in, int64_t stride_out,
+                        const int32_t *tokens, int64_t history, int64_t stride_tokens, const int32_t *lens,
+                        const int32_t *prompt_lens, const float *repetition, const float *frequency,
+                        const float *presence, const int32_t *bias_ids, const float *bias_values, int64_t num_biases,
+                        int64_t stride_bias, const int32_t *mask, int64_t stride_mask, int dtype, int variant, void *stream);
 
 /* ---- test hook ---------------------------------------------------------------------------- */
 
