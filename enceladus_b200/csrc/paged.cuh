@@ -50,7 +50,7 @@ static inline int check_cache(const enc_paged_cache &c, const char *me) {
 // Tokens that a row of the block table can address (positions are 32-bit).
 static inline int64_t paged_capacity(const enc_paged_cache &c) {
     const int64_t n = c.table_width * c.page_size;  // both below 2^31
-    return n < 0x7fffffffLL ? n : 0x7fffffffLL;
+    return n < 0x7fffff00LL ? n : 0x7fffff00LL;  // (room for the last tile in 32 bits)
 }
 
 #ifdef __CUDACC__

@@ -1,202 +1,12 @@
-// Attention of one new token per sequence over a paged key-value cache, split over the cache's length and joined.
-//
-// Mathematics: for a query row, s_j = q . k_j * sm_scale * log2(e); one pass over the keys keeps the running maximum m, the
-// sum l = sum_j 2^(s_j - m) and O = sum_j 2^(s_j - m) v_j, all float32.  Two pieces (m1, l1, O1), (m2, l2, O2) of a row join
-// to m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m) and the same for O, in any split.  o = O / l,
-// lse = (m + log2 l) ln 2.  A piece whose scores are all -inf has m = -inf and counts with weight zero.
-//
-// What bounds it: each key and value is read once and used by the query heads that share it, a handful of operations per
-// byte, so the bound is HBM bandwidth; with few or short sequences, latency.
-//
-// Split: the work is a line of 64-key tiles (sequence by sequence, kv head by kv head), dealt out in equal contiguous
-// runs over a grid that fills the GPU once.  Every CTA finds its run from seq_lens by a scan over the batch, so ragged
-// lengths, one long sequence and many short ones all load every SM alike, and nothing about the lengths has to reach
-// the host.  A row that ends inside a run is finished there; the up to two pieces of a run that belong to rows cut by
-// its ends go to a workspace and a second, overlapped launch joins them in order (no atomics: the result does not depend
-// on timing).
-#include "paged.cuh"
+// Attention of one new token per sequence over a paged key-value cache: the CUDA-core kernel, the join of split rows and the
+// entry points.  Mathematics, bound and split are in paged_attention.cuh.
+#include "paged_attention.cuh"
+
+#include <type_traits>
 
 namespace enc {
+using namespace paged;
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int THREADS = 128, WARPS = THREADS / 32;
-constexpr int TILE = 64;          // keys of a tile
-constexpr int MAX_HEAD_DIM = 256;
-
-struct PagedArgs {
-    const void *q, *k, *v;
-    void *o;
-    float *lse;
-    const int32_t *block_table, *seq_lens;
-    int4 *headers;   // per CTA: the row group that its last piece begins {first query row, rows, last CTA of it, -}
-    float *slots;    // per CTA two pieces of `rows` x (head_dim + 2) floats: O, m, l
-    int64_t sq_s, sq_h, so_s, so_h, sk_p, sk_h, sk_t, sv_p, sv_h, sv_t, s_table;
-    int64_t num_seqs, num_pages, capacity, window;
-    int q_heads, head_dim, group, row_groups;  // query rows per kv head; row groups (of the kernel's row count) per kv head
-    int units;                                 // row groups per sequence: kv_heads * row_groups
-    int min_run;                               // tiles a run has at least
-    float scale;                               // sm_scale * log2(e)
-    FastDiv page_size;
-};
-
-// ---- schedule ------------------------------------------------------------------------------------
-// Keys of sequence b that its row looks at: the first key and how many.
-__device__ __forceinline__ int keys_of(const PagedArgs &a, int64_t b, int &first) {
-    int n = a.seq_lens[b];
-    if (n < 0 || n > a.capacity) {
-        atomicExch(&g_bad_index, 1u);
-        n = n < 0 ? 0 : (int)a.capacity;
-    }
-    first = a.window > 0 && n > a.window ? n - (int)a.window : 0;
-    return n - first;
-}
-__device__ __forceinline__ int64_t tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
-
-struct Run {
-    int64_t seq, at;      // first sequence, first tile inside the sequence's units
-    int64_t begin, end;   // tiles on the line
-    int64_t run;          // tiles of a full run
-};
-
-// Every thread of the CTA returns the CTA's run of tiles.  The sequences are dealt to the threads in contiguous pieces;
-// the thread whose piece holds the run's first tile finds the sequence.
-__device__ __forceinline__ Run find_run(const PagedArgs &a) {
-    __shared__ int64_t warp_total[WARPS], found[2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t per = (a.num_seqs + THREADS - 1) / THREADS;
-    const int64_t b0 = threadIdx.x * per, b1 = b0 + per < a.num_seqs ? b0 + per : a.num_seqs;
-    int64_t mine = 0;
-    int first;
-    for (int64_t b = b0; b < b1; ++b) mine += tiles_of(keys_of(a, b, first));
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-    }
-    if (lane == 31) warp_total[warp] = upto;
-    __syncthreads();
-    int64_t total = 0, before = upto - mine;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) before += warp_total[w];
-        total += warp_total[w];
-    }
-    total *= a.units;
-    Run r;
-    r.run = (total + gridDim.x - 1) / gridDim.x;
-    if (r.run < a.min_run) r.run = a.min_run;
-    r.begin = blockIdx.x * r.run;
-    r.end = r.begin + r.run < total ? r.begin + r.run : total;
-    r.seq = r.at = 0;
-    if (r.begin >= r.end) return r;  // (the same for all threads: begin and end depend on the block alone)
-    if (before * a.units <= r.begin && r.begin < (before + mine) * a.units) {
-        int64_t at = r.begin - before * a.units;
-        for (int64_t b = b0; b < b1; ++b) {
-            const int64_t t = tiles_of(keys_of(a, b, first)) * a.units;
-            if (at < t) {
-                found[0] = b;
-                found[1] = at;
-                break;
-            }
-            at -= t;
-        }
-    }
-    __syncthreads();
-    r.seq = found[0];
-    r.at = found[1];
-    return r;
-}
-
-__device__ __forceinline__ float *slot_of(const PagedArgs &a, int64_t cta, int which, int rows) {
-    return a.slots + (2 * cta + which) * rows * (int64_t)(a.head_dim + 2);
-}
-
-// A piece's rows, one partial result per warp in shared memory (O unnormalised [WARPS][ROWS][stride], m and l [WARPS][ROWS]),
-// joined and written: to the output when the piece is the whole row, to `slot` otherwise.
-template <typename T, int ROWS>
-__device__ __forceinline__ void write_piece(const PagedArgs &a, const float *so, int stride, const float (*sm)[ROWS], const float (*sl)[ROWS],
-                                            int rows, int64_t seq, int first_head, float *slot) {
-    T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s;
-    for (int i = threadIdx.x; i < rows * a.head_dim; i += THREADS) {
-        const int r = i / a.head_dim, d = i - r * a.head_dim;
-        float m = sm[0][r];
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) m = fmaxf(m, sm[w][r]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float c = fast_exp2(sm[w][r] - base);
-            l = fmaf(sl[w][r], c, l);
-            x = fmaf(so[(w * ROWS + r) * stride + d], c, x);
-        }
-        if (slot) {
-            slot[r * (a.head_dim + 2) + d] = x;
-            if (d == 0) {
-                slot[r * (a.head_dim + 2) + a.head_dim] = m;
-                slot[r * (a.head_dim + 2) + a.head_dim + 1] = l;
-            }
-        } else {
-            o[(first_head + r) * a.so_h + d] = from_f32<T>(l == 0.0f ? 0.0f : __fdiv_rn(x, l));
-            if (d == 0 && a.lse) a.lse[seq * a.q_heads + first_head + r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
-        }
-    }
-}
-
-// Walks over the CTA's run: process(seq, kv head, first query head, rows, first key, keys, tile range, slot or NULL) per
-// piece.  Also writes the header that the join reads, and the rows of sequences without keys.
-template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk_run(const PagedArgs &a, F process) {
-    const Run run = find_run(a);
-    if (threadIdx.x == 0 && a.headers) a.headers[blockIdx.x].y = 0;
-    int64_t seq = run.seq, at = run.at;
-    for (int64_t pos = run.begin; pos < run.end;) {
-        int first;
-        const int keys = keys_of(a, seq, first);
-        const int64_t tiles = tiles_of(keys);
-        if (at >= tiles * a.units) {
-            at -= tiles * a.units;  // (zero: a sequence's tiles are walked to their end)
-            ++seq;
-            continue;
-        }
-        const int unit = (int)(at / tiles), t0 = (int)(at - unit * tiles);
-        const int t1 = tiles - t0 < run.end - pos ? (int)tiles : t0 + (int)(run.end - pos);
-        const int kv_head = unit / a.row_groups, rg = unit - kv_head * a.row_groups;
-        const int rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
-        const int first_head = kv_head * a.group + rg * ROWS;
-        float *slot = nullptr;
-        if (t0 > 0) {
-            slot = slot_of(a, blockIdx.x, 0, ROWS);
-        } else if (t1 < tiles) {
-            slot = slot_of(a, blockIdx.x, 1, ROWS);
-            if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), (int)((pos + tiles - 1) / run.run), 0);
-        }
-        process(seq, kv_head, first_head, rows, first, keys, t0, t1, slot);
-        pos += t1 - t0;
-        at += t1 - t0;
-    }
-    T *o = reinterpret_cast<T *>(a.o);
-    for (int64_t b = blockIdx.x; b < a.num_seqs; b += gridDim.x) {  // rows without keys
-        int first;
-        if (keys_of(a, b, first) > 0) continue;
-        for (int i = threadIdx.x; i < a.q_heads * a.head_dim; i += THREADS) {
-            const int h = i / a.head_dim, d = i - h * a.head_dim;
-            o[b * a.so_s + h * a.so_h + d] = from_f32<T>(0.0f);
-            if (d == 0 && a.lse) a.lse[b * a.q_heads + h] = -INFINITY;
-        }
-    }
-}
-
-// Where key `pos` of sequence seq lives: its page and its row in it; false (and the error word) if the page is out of range.
-__device__ __forceinline__ bool locate(const PagedArgs &a, int64_t seq, int pos, int64_t &page, int &row) {
-    const uint32_t pi = a.page_size.div((uint32_t)pos);
-    row = pos - (int)(pi * a.page_size.d);
-    page = a.block_table[seq * a.s_table + pi];
-    if (page >= 0 && page < a.num_pages) return true;
-    atomicExch(&g_bad_index, 1u);
-    return false;
-}
 
 // ---- join ------------------------------------------------------------------------------------------
 // One CTA per (run, row): where a run's last piece begins a row group, the pieces of that group are that piece and the first
@@ -365,13 +175,21 @@ template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bound
                 }
         }
         __syncthreads();
-        write_piece<T, ROWS>(a, so, MAX_HEAD_DIM, sm, sl, rows, seq, first_head, slot);
+        write_piece<T, ROWS>(a, so, ROWS * MAX_HEAD_DIM, MAX_HEAD_DIM, sm, sl, rows, seq, first_head, slot);
         __syncthreads();
     });
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-enum { V_CORES = 0, VARIANTS = 1 };
+enum { V_TENSOR = 0, V_CORES = 1, VARIANTS = 2 };
+
+// The tensor-core kernels take 16-bit types, head dimensions they are instantiated for, and 16-byte rows in the cache.
+bool tensor_ok(const enc_paged_cache &c, int dtype) {
+    if (dtype_size(dtype) != 2 || mma_ctas_per_sm(c.head_dim) == 0 || !aligned16(c.k) || !aligned16(c.v)) return false;
+    for (int64_t s : {c.k_stride_page, c.k_stride_head, c.k_stride_token, c.v_stride_page, c.v_stride_head, c.v_stride_token})
+        if (s % 8) return false;
+    return true;
+}
 
 struct Plan {
     int variant, rows, row_groups, grid;
@@ -379,29 +197,41 @@ struct Plan {
 };
 
 // Which kernel, how many query rows it takes at a time, how many CTAs, and the bytes for pieces.
-int make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant, Plan &p) {
+void make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant, Plan &p) {
     const int group = (int)(q_heads / c.kv_heads);
-    p.variant = V_CORES;
-    p.rows = group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
-    const int per_sm = 4;
+    p.variant = variant >= 0 ? variant : tensor_ok(c, dtype) ? V_TENSOR : V_CORES;
+    p.rows = p.variant == V_TENSOR ? MMA_ROWS : group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
+    const int per_sm = p.variant == V_TENSOR ? mma_ctas_per_sm(c.head_dim) : 4;
     p.row_groups = (int)cdiv(group, p.rows);
     const int64_t most = c.num_seqs * c.kv_heads * p.row_groups * cdiv(paged_capacity(c), TILE);  // tiles if every row is full
     const int64_t fill = (int64_t)device_props().sm_count * per_sm;
     p.grid = (int)(most < fill ? (most > 0 ? most : 1) : fill);
     // sequences of one tile are never cut
     p.work = paged_capacity(c) <= TILE ? 0 : (int64_t)p.grid * 16 + 2 * (int64_t)p.grid * p.rows * (c.head_dim + 2) * 4;
-    return 0;
+}
+
+template <typename T, int ROWS> void launch_join(const PagedArgs &a, int grid, cudaStream_t st) {
+    const int rows = a.group < ROWS ? a.group : ROWS;
+    if (a.headers) launch_overlapped(join_kernel<T, ROWS>, dim3(grid, rows), dim3(THREADS), 0, st, a);
 }
 
 template <typename T, int CH, int ROWS>
 void launch_simple(const PagedArgs &a, int grid, bool vec, cudaStream_t st) {
     if (vec) launch_overlapped(paged_simple_kernel<T, CH, ROWS, true>, dim3(grid), dim3(THREADS), 0, st, a);
     else launch_overlapped(paged_simple_kernel<T, CH, ROWS, false>, dim3(grid), dim3(THREADS), 0, st, a);
-    if (a.headers) launch_overlapped(join_kernel<T, ROWS>, dim3(grid, ROWS), dim3(THREADS), 0, st, a);
+    launch_join<T, ROWS>(a, grid, st);
 }
 
 template <typename T> int launch_paged(const PagedArgs &a, const Plan &p, cudaStream_t st) {
     note_indexed_launch();
+    if constexpr (sizeof(T) == 2) {
+        if (p.variant == V_TENSOR) {
+            const int rc = launch_mma(a, std::is_same<T, __half>::value ? ENC_F16 : ENC_BF16, p.grid, st);
+            if (rc != ENC_OK) return rc;
+            launch_join<T, MMA_ROWS>(a, p.grid, st);
+            return check_launch("enc_paged_attention");
+        }
+    }
     const int nv = 4;
     bool vec = a.head_dim % nv == 0;
     for (const void *x : {a.q, a.k, a.v}) vec = vec && reinterpret_cast<uintptr_t>(x) % (nv * sizeof(T)) == 0;
@@ -428,15 +258,19 @@ int check_paged(const enc_paged_cache *c, int64_t q_heads, int dtype, int varian
     if (c->head_dim > MAX_HEAD_DIM) return fail(ENC_ERR_UNSUPPORTED, "%s: head_dim %lld > %d", me, (long long)c->head_dim, MAX_HEAD_DIM);
     if (q_heads < 1 || q_heads % c->kv_heads) return fail(ENC_ERR_BAD_ARG, "%s: %lld query heads over %lld kv heads", me, (long long)q_heads, (long long)c->kv_heads);
     if (q_heads > 0xffff) return fail(ENC_ERR_UNSUPPORTED, "%s: more than 65535 query heads", me);
+    if (variant == V_TENSOR && !tensor_ok(*c, dtype))
+        return fail(ENC_ERR_UNSUPPORTED, "%s: variant %d needs float16 or bfloat16, another head_dim, or 16-byte aligned cache rows", me, variant);
     return 0;
 }
 
 }  // namespace
 
-unsigned int take_bad_index_paged_attention() { return take_bad_index_word(); }
+unsigned int take_bad_index_paged_mma();
+unsigned int take_bad_index_paged_attention() { return take_bad_index_word() | take_bad_index_paged_mma(); }
 int paged_attention_variants() { return VARIANTS; }
-void paged_attention_variant_info(int, char *out, size_t n) {
-    snprintf(out, n, "CUDA cores, eight lanes per key, keys and values straight to registers");
+void paged_attention_variant_info(int v, char *out, size_t n) {
+    if (v == V_TENSOR) snprintf(out, n, "mma m16n8k16, 16 query rows, 16 keys per warp and step, keys and values through a cp.async ring");
+    else snprintf(out, n, "CUDA cores, eight lanes per key, keys and values straight to registers");
 }
 
 }  // namespace enc

@@ -402,10 +402,8 @@ def _paged_attention(a, grid, variant, stream):
     _need(a, N.F32, "lse_ptr")
     cache, q_heads = _paged_cache(a, grid[0]), int(a["Q_HEADS"])
     nbytes = N.load().enc_paged_attention_work_bytes(cache, q_heads, dt, variant)
-    if nbytes < 0:
-        N.check(N.ERR_BAD_ARG)
     work = None
-    if nbytes:
+    if nbytes > 0:  # (a negative answer is a refusal, which the launch itself reports)
         torch = interop._torch()
         work = torch.empty(nbytes, dtype=torch.uint8, device=a["q_ptr"].device)
     N.call("enc_paged_attention", cache, _ptr(a["q_ptr"]), _ptr(a["o_ptr"]), _opt(a["lse_ptr"]), _ptr(a["seq_lens_ptr"]), q_heads,
