@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -44,13 +45,11 @@ class DeviceInfo(C.Structure):
                 ("global_mem", C.c_uint64), ("name", C.c_char * 128)]
 
 
-class PagedCache(C.Structure):
-    """`enc_paged_cache`: a paged key-value cache and its block table, as the native entry points take it."""
-
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("block_table", C.c_void_p),
-                *((n, C.c_int64) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "num_seqs", "table_width", "stride_table",
-                                           "k_stride_page", "k_stride_head", "k_stride_token",
-                                           "v_stride_page", "v_stride_head", "v_stride_token"))]
+# enc_paged_cache: three pointers and thirteen 64-bit sizes, in the header's order.  Packed bytes cost a launch a fifth of what
+# filling a ctypes structure does.
+PAGED_CACHE_FIELDS = ("k", "v", "block_table", "num_pages", "page_size", "kv_heads", "head_dim", "num_seqs", "table_width", "stride_table",
+                      "k_stride_page", "k_stride_head", "k_stride_token", "v_stride_page", "v_stride_head", "v_stride_token")
+paged_cache = struct.Struct("=16q").pack
 
 
 _p, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -76,9 +75,9 @@ SIGNATURES: dict[str, list] = {
     "enc_matmul": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _p],
     "enc_matmul_int": [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _p],
     "enc_attention_fwd": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f, _i, _i, _i, _p],
-    "enc_append_kv": [C.POINTER(PagedCache)] + [_p] * 8 + [_i64] * 3 + [_i] + [_i64] * 10 + [_i, _i, _p],
-    "enc_paged_attention": [C.POINTER(PagedCache), _p, _p, _p, _p] + [_i64] * 5 + [_f, _i64, _p, _i64, _i, _i, _p],
-    "enc_paged_attention_work_bytes": [C.POINTER(PagedCache), _i64, _i, _i],
+    "enc_append_kv": [_p] + [_p] * 8 + [_i64] * 3 + [_i] + [_i64] * 10 + [_i, _i, _p],
+    "enc_paged_attention": [_p, _p, _p, _p, _p] + [_i64] * 5 + [_f, _i64, _p, _i64, _i, _i, _p],
+    "enc_paged_attention_work_bytes": [_p, _i64, _i, _i],
     "enc_penalize_logits": [_p, _p] + [_i64] * 4 + [_p, _i64, _i64] + [_p] * 7 + [_i64, _i64, _p, _i64, _i, _i, _p],
     "enc_test_fail_next": [_i],
     "enc_test_device_wait": [C.c_uint, _p],

@@ -11,11 +11,13 @@ A user's own copy of a reference example works the same way after `import encela
 from __future__ import annotations
 
 import math
+import os
 
 import numpy as np
 
 import enceladus_b200 as enceladus
 import enceladus_b200.language as tl
+from enceladus_b200.runtime import interop, registry
 from enceladus_b200.configs import attention_configs, matmul_configs
 
 
@@ -282,39 +284,60 @@ def cumsum(x, reverse: bool = False):
 
 
 # ---- the decoding step: paged key-value cache, attention of one new token, logits -----------------------
-def _no_overlap(x, what: str) -> None:
+# A step runs once per generated token and its kernels can be as short as a few microseconds, so these wrappers keep the host's
+# share small: plain checks, and with torch tensors on the current device one call into the library without the launch path's
+# bookkeeping (`_straight`).  Everything else (NumPy arrays, another device, a forced variant) goes through `kernel[grid](...)`.
+def _strides(x):
+    """Strides in elements."""
+    try:
+        return x.stride()
+    except AttributeError:
+        return enceladus.element_strides(x)
+
+
+def _straight(kernel, *arrays) -> int | None:
+    """The stream for a straight call into the library, or None if the launch has to take the general path."""
+    if kernel.variant is not None or kernel.interpret is not None or os.environ.get("ENCELADUS_INTERPRET"):
+        return None
+    return interop.direct_stream(*arrays)
+
+
+def _no_overlap(x, st, what: str) -> None:
     """Refuses an output whose elements share memory (an expanded view), where writes would meet."""
-    if any(n > 1 and s == 0 for n, s in zip(x.shape, enceladus.element_strides(x))):
+    if 0 in st and any(n > 1 and s == 0 for n, s in zip(x.shape, st)):
         raise ValueError(f"{what} is written, so its elements can't share memory (a stride is 0)")
 
 
 def _check_cache(k_cache, v_cache, block_table):
-    if len(k_cache.shape) != 4 or tuple(k_cache.shape) != tuple(v_cache.shape):
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must both have shape (pages, kv_heads, page_size, head_dim), but got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+                         f"{tuple(shape)} and {tuple(v_cache.shape)}")
     if len(block_table.shape) != 2:
         raise ValueError(f"block_table must have shape (sequences, pages per sequence), not {tuple(block_table.shape)}")
-    ks, vs = enceladus.element_strides(k_cache), enceladus.element_strides(v_cache)
-    ts = enceladus.element_strides(block_table)
-    for x, st, what in ((k_cache, ks, "k_cache"), (v_cache, vs, "v_cache"), (block_table, ts, "block_table")):
-        if x.shape[-1] > 1 and st[-1] != 1 and 0 not in x.shape:
-            raise ValueError(f"the last dimension of {what} must be contiguous")
+    ks, vs, ts = _strides(k_cache), _strides(v_cache), _strides(block_table)
+    if ks[3] != 1 or vs[3] != 1 or ts[1] != 1:
+        for x, st, what in ((k_cache, ks, "k_cache"), (v_cache, vs, "v_cache"), (block_table, ts, "block_table")):
+            if x.shape[-1] > 1 and st[-1] != 1 and 0 not in x.shape:
+                raise ValueError(f"the last dimension of {what} must be contiguous")
     return ks, vs, ts[0]
 
 
 def _check_heads(x, what: str, rows: int, head_dim: int, heads: int | None = None):
     """Strides of a (rows, heads, head_dim) array with contiguous heads."""
-    if len(x.shape) != 3 or x.shape[0] != rows or x.shape[2] != head_dim or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{what} must have shape ({rows}, {'heads' if heads is None else heads}, {head_dim}), not {tuple(x.shape)}")
-    st = enceladus.element_strides(x)
-    if head_dim > 1 and st[2] != 1 and 0 not in x.shape:
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what} must have shape ({rows}, {'heads' if heads is None else heads}, {head_dim}), not {tuple(shape)}")
+    st = _strides(x)
+    if st[2] != 1 and head_dim > 1 and 0 not in shape:
         raise ValueError(f"the last dimension of {what} must be contiguous")
     return st
 
 
 def _check_row(x, what: str, n: int) -> None:
-    if len(x.shape) != 1 or x.shape[0] != n or (n > 1 and enceladus.element_strides(x)[0] != 1):
-        raise ValueError(f"{what} must be contiguous with shape ({n},), not {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 1 or shape[0] != n or (n > 1 and _strides(x)[0] != 1):
+        raise ValueError(f"{what} must be contiguous with shape ({n},), not {tuple(shape)}")
 
 
 @enceladus.jit
@@ -350,8 +373,8 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_ids, positions, cos=None,
     k_st, v_st = _check_heads(k, "k", tokens, d, kv_heads), _check_heads(v, "v", tokens, d, kv_heads)
     _check_row(seq_ids, "seq_ids", tokens)
     _check_row(positions, "positions", tokens)
-    _no_overlap(k_cache, "k_cache")
-    _no_overlap(v_cache, "v_cache")
+    _no_overlap(k_cache, ks, "k_cache")
+    _no_overlap(v_cache, vs, "v_cache")
     q_st = o_st = (0, 0, 0)
     q_heads = 0
     if q is not None:
@@ -359,24 +382,32 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_ids, positions, cos=None,
         if q_out is None:
             q_out = enceladus.new_empty(q)
         o_st = _check_heads(q_out, "q_out", tokens, d, q_heads)
-        _no_overlap(q_out, "q_out")
+        _no_overlap(q_out, o_st, "q_out")
     elif q_out is not None:
         raise ValueError("q_out without q")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     n_positions = rot_dim = cos_st = 0
     if cos is not None:
-        if len(cos.shape) != 2 or tuple(cos.shape) != tuple(sin.shape) or 2 * cos.shape[1] > d:
+        shape = cos.shape
+        if len(shape) != 2 or shape != sin.shape or 2 * shape[1] > d:
             raise ValueError(f"cos and sin must both have shape (positions, rot_dim / 2) with rot_dim <= {d}, but got "
                              f"{tuple(cos.shape)} and {tuple(sin.shape)}")
-        c, s = enceladus.element_strides(cos), enceladus.element_strides(sin)
-        if c != s or (cos.shape[1] > 1 and c[1] != 1):
+        c = _strides(cos)
+        if c != _strides(sin) or (shape[1] > 1 and c[1] != 1):
             raise ValueError("cos and sin must have the same strides and contiguous rows")
-        n_positions, rot_dim, cos_st = cos.shape[0], 2 * cos.shape[1], c[0]
+        n_positions, rot_dim, cos_st = shape[0], 2 * shape[1], c[0]
         if not rot_dim:
             cos = sin = None
-    append_kv_kernel[(tokens,)](k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, block_table.shape[0],
-                                block_table.shape[1], st, pages, n_positions, k_st[0], k_st[1], v_st[0], v_st[1], q_st[0], q_st[1],
+    seqs, width = block_table.shape
+    stream = _straight(append_kv_kernel, k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin)
+    if stream is not None:
+        registry.append_kv(k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, tokens, seqs, width, st, pages,
+                           n_positions, k_st[:2], v_st[:2], q_st[:2], o_st[:2], cos_st, ks[:3], vs[:3], q_heads, kv_heads, d, rot_dim,
+                           page_size, 1 if interleaved else 0, -1, stream)
+        return q_out
+    append_kv_kernel[(tokens,)](k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, seqs, width, st, pages,
+                                n_positions, k_st[0], k_st[1], v_st[0], v_st[1], q_st[0], q_st[1],
                                 o_st[0], o_st[1], cos_st, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,
                                 KV_HEADS=kv_heads, HEAD_DIM=d, ROT_DIM=rot_dim, PAGE_SIZE=page_size, INTERLEAVED=interleaved)
     return q_out
@@ -419,11 +450,15 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale: float 
         raise ValueError(f"window can't be negative, but got {window}")
     if o is None:
         o = enceladus.new_empty(q)
-    else:
-        _no_overlap(o, "o")
     o_st = _check_heads(o, "o", seqs, d, q_heads)
+    _no_overlap(o, o_st, "o")
     scale = 1.0 / math.sqrt(d) if sm_scale is None else sm_scale
     lse = enceladus.new_empty(q, (seqs, q_heads), np.float32) if return_lse else None
+    stream = _straight(paged_attention_kernel, q, k_cache, v_cache, o, lse, block_table, seq_lens)
+    if stream is not None:
+        registry.paged_attention(q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, seqs, block_table.shape[1], st, pages,
+                                 q_st[:2], o_st[:2], ks[:3], vs[:3], q_heads, kv_heads, d, page_size, -1, stream)
+        return (o, lse) if return_lse else o
     paged_attention_kernel[(seqs,)](q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, block_table.shape[1], st, pages,
                                     q_st[0], q_st[1], o_st[0], o_st[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,
                                     KV_HEADS=kv_heads, HEAD_DIM=d, PAGE_SIZE=page_size)
@@ -457,26 +492,29 @@ def penalize_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition
     m, n = logits.shape
 
     def rows_of(x, what, cols=None):
-        if len(x.shape) != 2 or x.shape[0] != m or (cols is not None and x.shape[1] != cols):
-            raise ValueError(f"{what} must have shape ({m}, {'...' if cols is None else cols}), not {tuple(x.shape)}")
-        st = enceladus.element_strides(x)
-        if x.shape[1] > 1 and st[1] != 1:
+        shape = x.shape
+        if len(shape) != 2 or shape[0] != m or (cols is not None and shape[1] != cols):
+            raise ValueError(f"{what} must have shape ({m}, {'...' if cols is None else cols}), not {tuple(shape)}")
+        st = _strides(x)
+        if st[1] != 1 and shape[1] > 1:
             raise ValueError(f"the rows of {what} must be contiguous")
         return st[0]
 
     si = rows_of(logits, "logits")
     past = (tokens, lens, prompt_lens, repetition, frequency, presence)
-    if any(x is None for x in past) and any(x is not None for x in past):
-        raise ValueError("tokens, lens, prompt_lens, repetition, frequency and presence go together")
     history = stride_tokens = n_biases = stride_bias = stride_mask = 0
     if tokens is not None:
-        history, stride_tokens = tokens.shape[-1], rows_of(tokens, "tokens")
+        if lens is None or prompt_lens is None or repetition is None or frequency is None or presence is None:
+            raise ValueError("tokens, lens, prompt_lens, repetition, frequency and presence go together")
+        stride_tokens, history = rows_of(tokens, "tokens"), tokens.shape[1]
         for x, what in zip(past[1:], ("lens", "prompt_lens", "repetition", "frequency", "presence")):
             _check_row(x, what, m)
+    elif any(x is not None for x in past):
+        raise ValueError("tokens, lens, prompt_lens, repetition, frequency and presence go together")
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values go together")
     if bias_ids is not None:
-        n_biases, stride_bias = bias_ids.shape[-1], rows_of(bias_ids, "bias_ids")
+        stride_bias, n_biases = rows_of(bias_ids, "bias_ids"), bias_ids.shape[1]
         if rows_of(bias_values, "bias_values", n_biases) != stride_bias and m > 1:
             raise ValueError("bias_ids and bias_values must have the same strides")
     if mask is not None:
@@ -485,8 +523,13 @@ def penalize_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition
             stride_mask = mask.shape[1]
     if out is None:
         out = enceladus.new_empty(logits)
-    else:
-        _no_overlap(out, "out")
+    so = rows_of(out, "out", n)
+    _no_overlap(out, (so,), "out")
+    stream = _straight(penalize_logits_kernel, logits, out, *past, bias_ids, bias_values, mask)
+    if stream is not None and m:
+        registry.penalize_logits(logits, out, *past, bias_ids, bias_values, mask, m, n, si, so, history, stride_tokens, n_biases, stride_bias,
+                                 stride_mask, -1, stream)
+        return out
     penalize_logits_kernel[(m,)](logits, out, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, mask,
-                                 n, si, rows_of(out, "out", n), history, stride_tokens, n_biases, stride_bias, stride_mask)
+                                 n, si, so, history, stride_tokens, n_biases, stride_bias, stride_mask)
     return out

@@ -189,7 +189,26 @@ def async_numpy_enabled() -> bool:
 
 
 def current_stream() -> int:
-    return int(_torch().cuda.current_stream().cuda_stream)
+    """The CUDA stream that torch currently enqueues on, as an integer handle.
+
+    The raw getter costs a fraction of a microsecond, `torch.cuda.current_stream()` three."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(torch.cuda.current_device()) if raw is not None else int(torch.cuda.current_stream().cuda_stream)
+
+
+def direct_stream(*arrays: Any) -> int | None:
+    """The current stream if a launch over these arrays can go straight to the library: every array (None: left out) is a
+    torch tensor on the current CUDA device, so there is nothing to stage and no device to switch.  None otherwise."""
+    torch = _torch_mod
+    if torch is None or not torch.cuda.is_initialized():
+        return None
+    tensor = torch.Tensor
+    dev = torch._C._cuda_getDevice()
+    for a in arrays:
+        if a is not None and not (isinstance(a, tensor) and a.is_cuda and a.get_device() == dev):
+            return None
+    return current_stream()
 
 
 def _np_as_torch_view(a: np.ndarray):

@@ -345,70 +345,127 @@ def _attention_lse(a, grid, variant, stream):
 
 
 # ---- the decoding step: paged cache, attention of one new token, logits -----------------------------
+# Each of the three calls below takes device tensors and sizes; the launch path reaches it through the adapter under it, the
+# wrapper in ops.py directly when there is nothing to stage.
 def _opt(t: Any) -> int | None:
-    return None if t is None else int(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
-def _need(a: dict[str, Any], code: int, *names: str) -> None:
-    for n in names:
-        if a[n] is not None and _code(a[n]) != code:
-            raise TypeError(f"argument `{n}` must be {'int32' if code == N.I32 else 'float32'}, not {interop.element_dtype(a[n])}")
+def _float_code(what: str, **arrays: Any) -> int:
+    """The enc_dtype that all arrays share; a TypeError that names them otherwise."""
+    dtypes = {t.dtype for t in arrays.values() if t is not None}
+    if len(dtypes) == 1:
+        code = interop._TORCH_CODE.get(dtypes.pop())
+        if code is not None:
+            return code
+    raise TypeError(f"{what}: arguments {list(arrays)} must share one element type that the kernels support, but got "
+                    f"{ {n: str(t.dtype) for n, t in arrays.items() if t is not None} }")
 
 
-_CACHE_STRIDES = "stride_kp stride_kh stride_kt stride_vp stride_vh stride_vt"
+def _need(dtype: Any, **arrays: Any) -> None:
+    for n, t in arrays.items():
+        if t is not None and t.dtype is not dtype:
+            raise TypeError(f"argument `{n}` must be {str(dtype).removeprefix('torch.')}, not {t.dtype}")
 
 
-def _paged_cache(a: dict[str, Any], seqs: int) -> N.PagedCache:
-    return N.PagedCache(_ptr(a["k_cache_ptr"]), _ptr(a["v_cache_ptr"]), _ptr(a["block_table_ptr"]), int(a["n_pages"]), int(a["PAGE_SIZE"]),
-                        int(a["KV_HEADS"]), int(a["HEAD_DIM"]), seqs, int(a["table_width"]), int(a["stride_table"]), int(a["stride_kp"]),
-                        int(a["stride_kh"]), int(a["stride_kt"]), int(a["stride_vp"]), int(a["stride_vh"]), int(a["stride_vt"]))
+def append_kv(k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, tokens, n_seqs, table_width, stride_table,
+              n_pages, n_positions, k_st, v_st, q_st, o_st, stride_cos, kc_st, vc_st, q_heads, kv_heads, head_dim, rot_dim, page_size,
+              interleaved, variant, stream) -> None:
+    torch = interop._torch()
+    dt = k.dtype
+    if not (v.dtype is dt and k_cache.dtype is dt and v_cache.dtype is dt and (q is None or (q.dtype is dt and q_out.dtype is dt)) and dt in interop._TORCH_CODE):
+        _float_code("append_kv_kernel", k_ptr=k, v_ptr=v, q_ptr=q, q_out_ptr=q_out, k_cache_ptr=k_cache, v_cache_ptr=v_cache)
+    i32 = torch.int32
+    if not (block_table.dtype is i32 and seq_ids.dtype is i32 and positions.dtype is i32):
+        _need(i32, block_table_ptr=block_table, seq_ids_ptr=seq_ids, positions_ptr=positions)
+    if cos is not None:
+        _need(torch.float32, cos_ptr=cos, sin_ptr=sin)
+    cache = N.paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), n_pages, page_size, kv_heads, head_dim, n_seqs,
+                          table_width, stride_table, *kc_st, *vc_st)
+    N.check(N.load().enc_append_kv(cache, k.data_ptr(), v.data_ptr(), _opt(q), _opt(q_out), _opt(cos), _opt(sin), seq_ids.data_ptr(),
+                                   positions.data_ptr(), tokens, q_heads, rot_dim, interleaved, n_positions, *k_st, *v_st, *q_st, *o_st,
+                                   stride_cos, interop._TORCH_CODE[dt], variant, stream))
+
+
+def _ints(a: dict[str, Any], names: str) -> list[int]:
+    return [int(a[n]) for n in names.split()]
 
 
 # grid[0] = tokens.  The caches are written in place, so a NumPy cache is copied in and back whole.
 @register("append_kv_kernel",
           "k_ptr v_ptr q_ptr q_out_ptr k_cache_ptr v_cache_ptr block_table_ptr seq_ids_ptr positions_ptr cos_ptr sin_ptr "
           "n_seqs table_width stride_table n_pages n_positions stride_k_token stride_k_head stride_v_token stride_v_head "
-          "stride_q_token stride_q_head stride_o_token stride_o_head stride_cos " + _CACHE_STRIDES +
-          " Q_HEADS KV_HEADS HEAD_DIM ROT_DIM PAGE_SIZE INTERLEAVED",
+          "stride_q_token stride_q_head stride_o_token stride_o_head stride_cos stride_kp stride_kh stride_kt stride_vp stride_vh stride_vt "
+          "Q_HEADS KV_HEADS HEAD_DIM ROT_DIM PAGE_SIZE INTERLEAVED",
           "k_ptr v_ptr q_ptr q_out_ptr k_cache_ptr v_cache_ptr block_table_ptr seq_ids_ptr positions_ptr cos_ptr sin_ptr",
           "q_out_ptr k_cache_ptr v_cache_ptr", N.K_APPEND_KV, optional="q_ptr q_out_ptr cos_ptr sin_ptr")
 def _append_kv(a, grid, variant, stream):
-    names = ("k_ptr", "v_ptr", "k_cache_ptr", "v_cache_ptr")
-    if (a["q_ptr"] is None) != (a["q_out_ptr"] is None):
-        raise TypeError("append_kv_kernel: `q_ptr` and `q_out_ptr` go together")
-    if a["q_ptr"] is not None:
-        names += ("q_ptr", "q_out_ptr")
-    dt = _same_dtype(a, *names)
-    _need(a, N.I32, "block_table_ptr", "seq_ids_ptr", "positions_ptr")
-    _need(a, N.F32, "cos_ptr", "sin_ptr")
-    N.call("enc_append_kv", _paged_cache(a, int(a["n_seqs"])), _ptr(a["k_ptr"]), _ptr(a["v_ptr"]), _opt(a["q_ptr"]), _opt(a["q_out_ptr"]),
-           _opt(a["cos_ptr"]), _opt(a["sin_ptr"]), _ptr(a["seq_ids_ptr"]), _ptr(a["positions_ptr"]), grid[0], int(a["Q_HEADS"]),
-           int(a["ROT_DIM"]), int(bool(a["INTERLEAVED"])), int(a["n_positions"]), int(a["stride_k_token"]), int(a["stride_k_head"]),
-           int(a["stride_v_token"]), int(a["stride_v_head"]), int(a["stride_q_token"]), int(a["stride_q_head"]),
-           int(a["stride_o_token"]), int(a["stride_o_head"]), int(a["stride_cos"]), dt, variant, stream)
+    for x, y in (("q_ptr", "q_out_ptr"), ("cos_ptr", "sin_ptr")):
+        if (a[x] is None) != (a[y] is None):
+            raise TypeError(f"append_kv_kernel: `{x}` and `{y}` go together")
+    append_kv(a["k_ptr"], a["v_ptr"], a["q_ptr"], a["q_out_ptr"], a["k_cache_ptr"], a["v_cache_ptr"], a["block_table_ptr"], a["seq_ids_ptr"],
+              a["positions_ptr"], a["cos_ptr"], a["sin_ptr"], grid[0], *_ints(a, "n_seqs table_width stride_table n_pages n_positions"),
+              _ints(a, "stride_k_token stride_k_head"), _ints(a, "stride_v_token stride_v_head"), _ints(a, "stride_q_token stride_q_head"),
+              _ints(a, "stride_o_token stride_o_head"), int(a["stride_cos"]), _ints(a, "stride_kp stride_kh stride_kt"),
+              _ints(a, "stride_vp stride_vh stride_vt"), *_ints(a, "Q_HEADS KV_HEADS HEAD_DIM ROT_DIM PAGE_SIZE"), int(bool(a["INTERLEAVED"])),
+              variant, stream)
 
 
-# grid[0] = sequences.  The buffer for split rows comes from torch's caching allocator on the launch's stream: nothing is
-# shared with other launches, and a captured launch keeps the one it was captured with.
+def paged_attention(q, k_cache, v_cache, o, lse, block_table, seq_lens, sm_scale, window, seqs, table_width, stride_table, n_pages, q_st, o_st,
+                    kc_st, vc_st, q_heads, kv_heads, head_dim, page_size, variant, stream) -> None:
+    """The buffer for split rows comes from torch's caching allocator on the launch's stream: nothing is shared with other
+    launches, and a captured launch keeps the one it was captured with."""
+    torch = interop._torch()
+    dt = q.dtype
+    if not (k_cache.dtype is dt and v_cache.dtype is dt and o.dtype is dt and dt in interop._TORCH_CODE):
+        _float_code("paged_attention_kernel", q_ptr=q, k_cache_ptr=k_cache, v_cache_ptr=v_cache, o_ptr=o)
+    i32 = torch.int32
+    if not (block_table.dtype is i32 and seq_lens.dtype is i32):
+        _need(i32, block_table_ptr=block_table, seq_lens_ptr=seq_lens)
+    if lse is not None:
+        _need(torch.float32, lse_ptr=lse)
+    cache = N.paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), n_pages, page_size, kv_heads, head_dim, seqs,
+                          table_width, stride_table, *kc_st, *vc_st)
+    code, lib = interop._TORCH_CODE[dt], N.load()
+    nbytes = lib.enc_paged_attention_work_bytes(cache, q_heads, code, variant)
+    work = None
+    if nbytes > 0:  # (a negative answer is a refusal, which the launch itself reports)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    N.check(lib.enc_paged_attention(cache, q.data_ptr(), o.data_ptr(), _opt(lse), seq_lens.data_ptr(), q_heads, *q_st, *o_st, sm_scale, window,
+                                    _opt(work), nbytes, code, variant, stream))
+
+
+# grid[0] = sequences
 @register("paged_attention_kernel",
           "q_ptr k_cache_ptr v_cache_ptr o_ptr lse_ptr block_table_ptr seq_lens_ptr sm_scale window table_width stride_table n_pages "
-          "stride_qs stride_qh stride_os stride_oh " + _CACHE_STRIDES + " Q_HEADS KV_HEADS HEAD_DIM PAGE_SIZE",
+          "stride_qs stride_qh stride_os stride_oh stride_kp stride_kh stride_kt stride_vp stride_vh stride_vt Q_HEADS KV_HEADS HEAD_DIM PAGE_SIZE",
           "q_ptr k_cache_ptr v_cache_ptr o_ptr lse_ptr block_table_ptr seq_lens_ptr", "o_ptr lse_ptr", N.K_PAGED_ATTENTION,
           extents=lambda a, g: {"lse_ptr": g[0] * int(a["Q_HEADS"]), **({"o_ptr": g[0] * int(a["Q_HEADS"]) * int(a["HEAD_DIM"])} if int(a["stride_oh"]) == int(a["HEAD_DIM"]) and int(a["stride_os"]) == int(a["Q_HEADS"]) * int(a["HEAD_DIM"]) else {})},
           optional="lse_ptr")
 def _paged_attention(a, grid, variant, stream):
-    dt = _same_dtype(a, "q_ptr", "k_cache_ptr", "v_cache_ptr", "o_ptr")
-    _need(a, N.I32, "block_table_ptr", "seq_lens_ptr")
-    _need(a, N.F32, "lse_ptr")
-    cache, q_heads = _paged_cache(a, grid[0]), int(a["Q_HEADS"])
-    nbytes = N.load().enc_paged_attention_work_bytes(cache, q_heads, dt, variant)
-    work = None
-    if nbytes > 0:  # (a negative answer is a refusal, which the launch itself reports)
-        torch = interop._torch()
-        work = torch.empty(nbytes, dtype=torch.uint8, device=a["q_ptr"].device)
-    N.call("enc_paged_attention", cache, _ptr(a["q_ptr"]), _ptr(a["o_ptr"]), _opt(a["lse_ptr"]), _ptr(a["seq_lens_ptr"]), q_heads,
-           int(a["stride_qs"]), int(a["stride_qh"]), int(a["stride_os"]), int(a["stride_oh"]), float(a["sm_scale"]), int(a["window"]),
-           _opt(work), nbytes, dt, variant, stream)
+    paged_attention(a["q_ptr"], a["k_cache_ptr"], a["v_cache_ptr"], a["o_ptr"], a["lse_ptr"], a["block_table_ptr"], a["seq_lens_ptr"],
+                    float(a["sm_scale"]), int(a["window"]), grid[0], *_ints(a, "table_width stride_table n_pages"), _ints(a, "stride_qs stride_qh"),
+                    _ints(a, "stride_os stride_oh"), _ints(a, "stride_kp stride_kh stride_kt"), _ints(a, "stride_vp stride_vh stride_vt"),
+                    *_ints(a, "Q_HEADS KV_HEADS HEAD_DIM PAGE_SIZE"), variant, stream)
+
+
+def penalize_logits(logits, out, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, mask, rows, vocab, stride_in,
+                    stride_out, history, stride_tokens, n_biases, stride_bias, stride_mask, variant, stream) -> None:
+    torch = interop._torch()
+    dt = logits.dtype
+    if out.dtype is not dt or dt not in interop._TORCH_CODE:
+        _float_code("penalize_logits_kernel", logits_ptr=logits, out_ptr=out)
+    i32, f32 = torch.int32, torch.float32
+    for t in (tokens, lens, prompt_lens, bias_ids, mask):
+        if t is not None and t.dtype is not i32:
+            _need(i32, tokens_ptr=tokens, lens_ptr=lens, prompt_lens_ptr=prompt_lens, bias_ids_ptr=bias_ids, mask_ptr=mask)
+    for t in (repetition, frequency, presence, bias_values):
+        if t is not None and t.dtype is not f32:
+            _need(f32, repetition_ptr=repetition, frequency_ptr=frequency, presence_ptr=presence, bias_values_ptr=bias_values)
+    N.check(N.load().enc_penalize_logits(logits.data_ptr(), out.data_ptr(), rows, vocab, stride_in, stride_out, _opt(tokens), history,
+                                         stride_tokens, _opt(lens), _opt(prompt_lens), _opt(repetition), _opt(frequency), _opt(presence),
+                                         _opt(bias_ids), _opt(bias_values), n_biases, stride_bias, _opt(mask), stride_mask,
+                                         interop._TORCH_CODE[dt], variant, stream))
 
 
 # grid[0] = rows
@@ -420,11 +477,6 @@ def _paged_attention(a, grid, variant, stream):
           extents=lambda a, g: {"out_ptr": g[0] * int(a["vocab"])} if int(a["stride_out"]) == int(a["vocab"]) else {},
           optional="tokens_ptr lens_ptr prompt_lens_ptr repetition_ptr frequency_ptr presence_ptr bias_ids_ptr bias_values_ptr mask_ptr")
 def _penalize_logits(a, grid, variant, stream):
-    dt = _same_dtype(a, "logits_ptr", "out_ptr")
-    _need(a, N.I32, "tokens_ptr", "lens_ptr", "prompt_lens_ptr", "bias_ids_ptr", "mask_ptr")
-    _need(a, N.F32, "repetition_ptr", "frequency_ptr", "presence_ptr", "bias_values_ptr")
-    N.call("enc_penalize_logits", _ptr(a["logits_ptr"]), _ptr(a["out_ptr"]), grid[0], int(a["vocab"]), int(a["stride_in"]),
-           int(a["stride_out"]), _opt(a["tokens_ptr"]), int(a["history"]), int(a["stride_tokens"]), _opt(a["lens_ptr"]),
-           _opt(a["prompt_lens_ptr"]), _opt(a["repetition_ptr"]), _opt(a["frequency_ptr"]), _opt(a["presence_ptr"]),
-           _opt(a["bias_ids_ptr"]), _opt(a["bias_values_ptr"]), int(a["n_biases"]), int(a["stride_bias"]), _opt(a["mask_ptr"]),
-           int(a["stride_mask"]), dt, variant, stream)
+    penalize_logits(*(a[n] for n in ("logits_ptr", "out_ptr", "tokens_ptr", "lens_ptr", "prompt_lens_ptr", "repetition_ptr", "frequency_ptr",
+                                     "presence_ptr", "bias_ids_ptr", "bias_values_ptr", "mask_ptr")), grid[0],
+                    *_ints(a, "vocab stride_in stride_out history stride_tokens n_biases stride_bias stride_mask"), variant, stream)

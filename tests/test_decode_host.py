@@ -6,6 +6,7 @@ import ctypes
 
 import numpy as np
 import pytest
+import torch
 
 from enceladus_b200 import _native as N
 from enceladus_b200 import ops
@@ -24,7 +25,7 @@ def cache(**kw):
     c = dict(k=16, v=16, block_table=16, num_pages=4, page_size=16, kv_heads=2, head_dim=64, num_seqs=3, table_width=5, stride_table=5,
              k_stride_page=2048, k_stride_head=1024, k_stride_token=64, v_stride_page=2048, v_stride_head=1024, v_stride_token=64)
     c.update(kw)
-    return N.PagedCache(**c)
+    return N.paged_cache(*(c[n] or 0 for n in N.PAGED_CACHE_FIELDS))
 
 
 def append(lib, c, *, k=16, v=16, q=None, q_out=None, cos=None, sin=None, ids=16, pos=16, tokens=2, q_heads=0, rot=0, n_pos=0, dtype=N.F32,
@@ -44,8 +45,8 @@ def logits(lib, *, x=16, out=16, rows=2, vocab=100, past=(None,) * 6, history=0,
 
 
 def test_struct_matches_the_header():
-    assert ctypes.sizeof(N.PagedCache) == 16 * 8
-    names = [n for n, _ in N.PagedCache._fields_]
+    assert len(cache()) == 16 * 8 and ctypes.sizeof(ctypes.c_void_p) == 8
+    names = list(N.PAGED_CACHE_FIELDS)
     text = (N.LIB_PATH.parents[2] / "include" / "enceladus_b200.h").read_text()
     body = text[text.index("typedef struct {\n    void *k, *v;"):text.index("} enc_paged_cache;")]
     import re
@@ -145,7 +146,11 @@ def test_append_wrapper_refusals():
         with pytest.raises(ValueError, match=match):
             ops.append_kv(**{**good, **change})
     with pytest.raises(TypeError, match="`positions_ptr` must be"):
-        registry._need({"positions_ptr": np.zeros(3, np.int64)}, N.I32, "positions_ptr")
+        registry._need(torch.int32, positions_ptr=torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(TypeError, match="share one element type"):
+        registry._float_code("x", k_ptr=torch.zeros(1), v_ptr=torch.zeros(1, dtype=torch.float16))
+    with pytest.raises(TypeError, match="share one element type"):
+        registry._float_code("x", k_ptr=torch.zeros(1, dtype=torch.float64))
 
 
 def test_attention_wrapper_refusals():
