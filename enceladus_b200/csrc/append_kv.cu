@@ -23,105 +23,159 @@ struct AppendArgs {
     int64_t ck_p, ck_h, ck_t, cv_p, cv_h, cv_t, s_table;
     int64_t num_seqs, num_pages, num_positions, capacity;
     int q_heads, kv_heads, head_dim, rot_dim;
+    bool angles_aligned;  // rows of cos and sin start on 16 bytes
     FastDiv page_size;
 };
 
-// One CTA per token.  VEC: 16-byte vectors (NV elements); else single elements.  An item is one place inside a head: a pair
-// of vectors that turn together (one vector of neighbouring pairs when INTERLEAVED), or a vector that is copied.
-template <typename T, bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
-    constexpr int NV = VEC ? Pack<T>::N : (INTERLEAVED ? 2 : 1);  // elements of an item's vector
-    constexpr int UN = 4;                                         // heads in flight per thread
-    constexpr int NC = INTERLEAVED ? (NV / 2 > 0 ? NV / 2 : 1) : NV;  // angles of an item
-    struct alignas(VEC ? 16 : sizeof(T)) Vec { T e[NV]; };
-    grid_dependency_wait();
-    const int64_t t = blockIdx.x;
-    const int seq = a.seq_ids[t], pos = a.positions[t];
-    const int turning = INTERLEAVED ? a.rot_dim / NV : a.rot_dim / 2 / NV;
-    const int tail = a.head_dim - a.rot_dim;  // copied elements behind the rotated ones
-    constexpr int CV = VEC ? NV : 1;          // elements of a copied vector
-    const int items = turning + tail / CV;
-    const int x = threadIdx.x % (items < THREADS ? items : THREADS);
-    const int y = threadIdx.x / (items < THREADS ? items : THREADS), ny = items < THREADS ? THREADS / items : 1;
-    const int heads = a.kv_heads + (a.q ? a.q_heads : 0);  // key heads first, then query heads
-
-    bool ok = seq >= 0;
-    int64_t page = 0;
-    int row = 0;
-    if (ok) {
-        ok = seq < a.num_seqs && pos >= 0 && pos < a.capacity && (a.rot_dim == 0 || pos < a.num_positions);
-        if (ok) {
-            const uint32_t pi = a.page_size.div((uint32_t)pos);
-            row = pos - (int)(pi * a.page_size.d);
-            page = a.block_table[seq * a.s_table + pi];
-            ok = page >= 0 && page < a.num_pages;
+template <int N> __device__ __forceinline__ void load_floats(const float *p, bool aligned, float (&f)[N]) {
+    if (N % 4 == 0 && aligned) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const float4 x = *reinterpret_cast<const float4 *>(p + 4 * i);
+            f[4 * i] = x.x; f[4 * i + 1] = x.y; f[4 * i + 2] = x.z; f[4 * i + 3] = x.w;
         }
-        if (!ok && threadIdx.x == 0) atomicExch(&g_bad_index, 1u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = p[i];
     }
-    if (!ok) return;
+}
 
+// N neighbouring elements: one 16-byte vector, or single elements where rows are not aligned for that.
+template <typename T, int N, bool VEC> struct Elems {
+    T e[N];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = p[i];
+    }
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = e[i];
+    }
+    __device__ __forceinline__ void get(float (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = to_f32(e[i]);
+    }
+    __device__ __forceinline__ void set(const float (&f)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = from_f32<T>(f[i]);
+    }
+};
+template <typename T, int N> struct Elems<T, N, true> {
+    uint4 v;
+    __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = v; }
+    __device__ __forceinline__ void get(float (&f)[N]) const { Pack<T>::unpack(v, f); }
+    __device__ __forceinline__ void set(const float (&f)[N]) { v = Pack<T>::pack(f); }
+};
+
+// One CTA per token.  VEC: 16-byte vectors (NV elements); else single elements.  An item is one place inside a head: a pair
+// of vectors that turn together (one vector of neighbouring pairs when INTERLEAVED), or a vector that is copied.  The loads
+// of a thread's first UN heads and of its first value vector are under way before the token's position, its page and its
+// angles have arrived: they are the longest chain (index -> page number, position -> cosines).
+template <typename T, bool VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(THREADS, 8) append_kernel(AppendArgs a) {
+    constexpr int NV = VEC ? Pack<T>::N : (INTERLEAVED ? 2 : 1);  // elements of an item's vector
+    constexpr int UN = 3;                                         // heads in flight per thread
+    constexpr int NC = INTERLEAVED ? NV / 2 : NV;                 // angles of an item
+    constexpr int CV = VEC ? NV : 1;                              // elements of a copied vector
+    using Vec = Elems<T, NV, VEC>;
+    using Copy = Elems<T, CV, VEC>;
+    const int64_t t = blockIdx.x;
+    const int turning = INTERLEAVED ? a.rot_dim / NV : a.rot_dim / 2 / NV;
+    const int items = turning + (a.head_dim - a.rot_dim) / CV;
+    const int nx = items < THREADS ? items : THREADS, ny = THREADS / nx;
+    const int x = threadIdx.x % nx, y = threadIdx.x / nx;
+    const int heads = a.kv_heads + (a.q ? a.q_heads : 0);  // key heads first, then query heads
+    const int vh = a.head_dim / CV, values = a.kv_heads * vh;
     const T *k = reinterpret_cast<const T *>(a.k) + t * a.sk_t, *v = reinterpret_cast<const T *>(a.v) + t * a.sv_t;
     const T *q = reinterpret_cast<const T *>(a.q) + t * a.sq_t;
     T *qo = reinterpret_cast<T *>(a.q_out) + t * a.so_t;
+    grid_dependency_wait();
+    const int seq = a.seq_ids[t], pos = a.positions[t];
+
+    Vec u[UN], w[UN];
+    auto load = [&](int it, int h0) {
+        const bool turn = it < turning;
+        const int off = turn ? it * NV : a.rot_dim + (it - turning) * CV;
+#pragma unroll
+        for (int j = 0; j < UN; ++j) {
+            const int h = h0 + j * ny;
+            if (h >= heads) continue;
+            const T *src = h < a.kv_heads ? k + h * a.sk_h : q + (h - a.kv_heads) * a.sq_h;
+            if (VEC || turn) u[j].load(src + off);
+            else reinterpret_cast<Copy &>(u[j]).load(src + off);
+            if (!INTERLEAVED && turn) w[j].load(src + off + a.rot_dim / 2);
+        }
+    };
+    auto value = [&](int i) {
+        Copy c;
+        c.load(v + (i / vh) * a.sv_h + (i % vh) * CV);
+        return c;
+    };
+    const bool mine = y < ny;
+    if (mine) load(x, y);
+    Copy first_value;
+    if (threadIdx.x < values) first_value = value(threadIdx.x);
+
+    if (seq < 0) return;  // padding
+    int64_t page = 0;
+    int row = 0;
+    bool ok = seq < a.num_seqs && pos >= 0 && pos < a.capacity && (a.rot_dim == 0 || pos < a.num_positions);
+    if (ok) {
+        const uint32_t pi = a.page_size.div((uint32_t)pos);
+        row = pos - (int)(pi * a.page_size.d);
+        page = a.block_table[seq * a.s_table + pi];
+        ok = page >= 0 && page < a.num_pages;
+    }
+    if (!ok) {
+        if (threadIdx.x == 0) atomicExch(&g_bad_index, 1u);
+        return;
+    }
     T *kc = reinterpret_cast<T *>(a.k_cache) + page * a.ck_p + row * a.ck_t;
     T *vc = reinterpret_cast<T *>(a.v_cache) + page * a.cv_p + row * a.cv_t;
 
-    if (y < ny) {
+    if (mine) {
         for (int it = x; it < items; it += THREADS) {
             const bool turn = it < turning;
             const int off = turn ? it * NV : a.rot_dim + (it - turning) * CV, off2 = off + a.rot_dim / 2;
             float cs[NC], sn[NC];
             if (turn) {
-                const float *c = a.cos + pos * a.s_cos + it * NC, *s = a.sin + pos * a.s_cos + it * NC;
-#pragma unroll
-                for (int e = 0; e < NC; ++e) {
-                    cs[e] = c[e];
-                    sn[e] = s[e];
-                }
+                load_floats<NC>(a.cos + pos * a.s_cos + it * NC, a.angles_aligned, cs);
+                load_floats<NC>(a.sin + pos * a.s_cos + it * NC, a.angles_aligned, sn);
             }
             for (int h0 = y; h0 < heads; h0 += ny * UN) {
-                Vec u[UN], w[UN];
-#pragma unroll
-                for (int j = 0; j < UN; ++j) {
-                    const int h = h0 + j * ny;
-                    if (h >= heads) continue;
-                    const T *src = h < a.kv_heads ? k + h * a.sk_h : q + (h - a.kv_heads) * a.sq_h;
-                    if (VEC || turn) u[j] = *reinterpret_cast<const Vec *>(src + off);
-                    else u[j].e[0] = src[off];
-                    if (!INTERLEAVED && turn) w[j] = *reinterpret_cast<const Vec *>(src + off2);
-                }
+                if (it != x || h0 != y) load(it, h0);
 #pragma unroll
                 for (int j = 0; j < UN; ++j) {
                     const int h = h0 + j * ny;
                     if (h >= heads) continue;
                     T *dst = h < a.kv_heads ? kc + h * a.ck_h : qo + (h - a.kv_heads) * a.so_h;
-                    if (turn) {
+                    if (!turn) {
+                        reinterpret_cast<const Copy &>(u[j]).store(dst + off);
+                        continue;
+                    }
+                    float fu[NV], fw[NV];
+                    u[j].get(fu);
+                    if (!INTERLEAVED) w[j].get(fw);
 #pragma unroll
-                        for (int e = 0; e < NC; ++e) {
-                            T &lo = INTERLEAVED ? u[j].e[(2 * e) % NV] : u[j].e[e];
-                            T &hi = INTERLEAVED ? u[j].e[(2 * e + 1) % NV] : w[j].e[e];
-                            const float fa = to_f32(lo), fb = to_f32(hi);
-                            lo = from_f32<T>(fmaf(fa, cs[e], -(fb * sn[e])));
-                            hi = from_f32<T>(fmaf(fb, cs[e], fa * sn[e]));
-                        }
-                        *reinterpret_cast<Vec *>(dst + off) = u[j];
-                        if (!INTERLEAVED) *reinterpret_cast<Vec *>(dst + off2) = w[j];
-                    } else if (VEC) {
-                        *reinterpret_cast<Vec *>(dst + off) = u[j];
-                    } else {
-                        dst[off] = u[j].e[0];
+                    for (int e = 0; e < NC; ++e) {
+                        float &lo = INTERLEAVED ? fu[(2 * e) % NV] : fu[e], &hi = INTERLEAVED ? fu[(2 * e + 1) % NV] : fw[e];
+                        const float x0 = lo, x1 = hi;
+                        lo = fmaf(x0, cs[e], -(x1 * sn[e]));
+                        hi = fmaf(x1, cs[e], x0 * sn[e]);
+                    }
+                    u[j].set(fu);
+                    u[j].store(dst + off);
+                    if (!INTERLEAVED) {
+                        w[j].set(fw);
+                        w[j].store(dst + off2);
                     }
                 }
             }
         }
     }
-    // values: plain copies
-    const int vh = a.head_dim / CV, n = a.kv_heads * vh;
-    struct alignas(VEC ? 16 : sizeof(T)) Copy { T e[CV]; };
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const int h = i / vh, c = (i - h * vh) * CV;
-        *reinterpret_cast<Copy *>(vc + h * a.cv_h + c) = *reinterpret_cast<const Copy *>(v + h * a.sv_h + c);
-    }
+    for (int i = threadIdx.x; i < values; i += THREADS)  // values: plain copies
+        (i < THREADS ? first_value : value(i)).store(vc + (i / vh) * a.cv_h + (i % vh) * CV);
 }
 
 template <typename T>
@@ -179,6 +233,7 @@ extern "C" int enc_append_kv(const enc_paged_cache *cache, const void *k, const 
     a.capacity = paged_capacity(*cache);
     a.q_heads = (int)q_heads; a.kv_heads = (int)cache->kv_heads; a.head_dim = (int)cache->head_dim; a.rot_dim = (int)rot_dim;
     a.page_size = FastDiv((uint32_t)cache->page_size);
+    a.angles_aligned = aligned16(cos) && aligned16(sin) && stride_cos % 4 == 0;
     // 16-byte vectors where every row starts on 16 bytes and no vector straddles the rotated part or its halves
     const int nv = 16 / (int)dtype_size(dtype);
     bool vec = cache->head_dim % nv == 0 && rot_dim % (interleaved ? nv : 2 * nv) == 0 && aligned16(k) && aligned16(v) &&

@@ -14,7 +14,6 @@ namespace enc {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MAX_TILE = 8192;                                         // tokens of a stretch at most (32 KB of counts)
 constexpr uint32_t IN_PROMPT = 1u << 31, HAS_BIAS = 1u << 30;          // above the count, which the history's length bounds
 constexpr uint32_t COUNT = HAS_BIAS - 1;
 
@@ -24,72 +23,145 @@ struct LogitsArgs {
     const int32_t *tokens, *lens, *prompt_lens, *bias_ids, *mask;
     const float *repetition, *frequency, *presence, *bias_values;
     int64_t vocab, s_in, s_out, s_tokens, s_bias, s_mask;
-    int history, biases, tile;
+    int history, biases;
 };
 
-template <typename T> __global__ void __launch_bounds__(THREADS) logits_kernel(LogitsArgs a) {
-    extern __shared__ uint32_t seen[];
-    grid_dependency_wait();
+// The logit of a token that its count word says something about.  Not inlined: it is rare, and 32 copies of it in the
+// streaming loop outgrow the instruction cache (0.4 of all stalls at 256 x 131072).
+__device__ __noinline__ float changed(float x, uint32_t w, float rep, float freq, float pres, const int32_t *ids, const float *values, int biases, int t) {
+    const uint32_t n = w & COUNT;
+    if (n || (w & IN_PROMPT)) x = x > 0.0f ? __fdiv_rn(x, rep) : x * rep;
+    if (n) x -= fmaf(freq, (float)n, pres);
+    if (w & HAS_BIAS) {
+        float b = 0.0f;
+        for (int i = 0; i < biases; ++i)
+            if (ids[i] == t) b += values[i];
+        x += b;
+    }
+    return x;
+}
+
+// VPT 16-byte vectors per thread: a stretch of VPT * THREADS vectors.  Stretches are cut so that the input's vectors are
+// aligned whatever the row's address: with `skew` elements of the row's first vector in front of the row, stretch i starts at
+// token i * TILE - skew.
+template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits_kernel(LogitsArgs a) {
+    constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
+    __shared__ __align__(16) uint32_t seen[TILE];
     const int64_t row = blockIdx.y;
-    const int v0 = blockIdx.x * a.tile, v1 = a.vocab - v0 < a.tile ? (int)a.vocab : v0 + a.tile;
-    for (int i = threadIdx.x; i < v1 - v0; i += THREADS) seen[i] = 0;
+    const T *in = reinterpret_cast<const T *>(a.in) + row * a.s_in;
+    T *out = reinterpret_cast<T *>(a.out) + row * a.s_out;
+    const int skew = (int)(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T)), vocab = (int)a.vocab;
+    const int v0 = (int)blockIdx.x * TILE - skew;  // token of seen[0]; negative in a skewed row's first stretch
+    if (v0 >= vocab) return;
+    const int lo = v0 < 0 ? 0 : v0, hi = v0 + TILE < vocab ? v0 + TILE : vocab;  // tokens of the stretch
+    const bool aligned_out = reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == skew;
+    const int32_t *mask = a.mask ? a.mask + row * a.s_mask : nullptr;
+    grid_dependency_wait();
+    // the logits are on their way while the history is counted
+    uint4 x[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int t = v0 + (j * THREADS + (int)threadIdx.x) * NV;
+        if (t >= 0 && t + NV <= vocab) {
+            x[j] = *reinterpret_cast<const uint4 *>(in + t);
+        } else {
+            T *e = reinterpret_cast<T *>(&x[j]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) e[i] = t + i >= 0 && t + i < vocab ? in[t + i] : from_f32<T>(0.0f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TILE / 4 / THREADS; ++i) reinterpret_cast<uint4 *>(seen)[i * THREADS + threadIdx.x] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     const bool reports = blockIdx.x == 0;  // one CTA per row reports what is out of range
+    bool bad = false;
     if (a.tokens) {
         int n = a.lens[row], prompt = a.prompt_lens[row];
-        if (n < 0 || n > a.history || prompt < 0 || prompt > n) {
-            if (reports && threadIdx.x == 0) atomicExch(&g_bad_index, 1u);
-            n = n < 0 ? 0 : n > a.history ? a.history : n;
-        }
+        bad = n < 0 || n > a.history || prompt < 0 || prompt > n;
+        n = n < 0 ? 0 : n > a.history ? a.history : n;
         rep = a.repetition[row];
         freq = a.frequency[row];
         pres = a.presence[row];
         const int32_t *tok = a.tokens + row * a.s_tokens;
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const int t = tok[i];
-            if (t >= v0 && t < v1) {
+        auto count = [&](int t, int i) {
+            if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
                 if (i < prompt) atomicOr(&seen[t - v0], IN_PROMPT);
                 else atomicAdd(&seen[t - v0], 1u);
-            } else if (reports && (t < 0 || t >= a.vocab)) {
-                atomicExch(&g_bad_index, 1u);
+            }
+        };
+        const int n4 = aligned16(tok) ? n / 4 : 0;
+        constexpr int UN = 4;  // vectors in flight per thread
+        for (int i = threadIdx.x; i < n4; i += UN * THREADS) {
+            int4 t[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) t[u] = i + u * THREADS < n4 ? reinterpret_cast<const int4 *>(tok)[i + u * THREADS] : make_int4(-1, -1, -1, -1);
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int at = 4 * (i + u * THREADS);
+                count(t[u].x, at);
+                count(t[u].y, at + 1);
+                count(t[u].z, at + 2);
+                count(t[u].w, at + 3);
             }
         }
+        for (int i = 4 * n4 + threadIdx.x; i < n; i += THREADS) count(tok[i], i);
+        if (reports)
+            for (int i = threadIdx.x; i < n; i += THREADS) bad |= (unsigned)tok[i] >= (unsigned)vocab;
     }
     const int32_t *ids = a.bias_ids + row * a.s_bias;
     const float *values = a.bias_values + row * a.s_bias;
     for (int i = threadIdx.x; i < a.biases; i += THREADS) {
         const int t = ids[i];
-        if (t >= v0 && t < v1) atomicOr(&seen[t - v0], HAS_BIAS);
-        else if (reports && (t < -1 || t >= a.vocab)) atomicExch(&g_bad_index, 1u);
+        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) atomicOr(&seen[t - v0], HAS_BIAS);
+        else if (t < -1 || t >= vocab) bad = true;
     }
+    if (bad && reports) atomicExch(&g_bad_index, 1u);
     __syncthreads();
-    const T *in = reinterpret_cast<const T *>(a.in) + row * a.s_in;
-    T *out = reinterpret_cast<T *>(a.out) + row * a.s_out;
-    const int32_t *mask = a.mask ? a.mask + row * a.s_mask : nullptr;
-    for (int t = v0 + threadIdx.x; t < v1; t += THREADS) {
-        float x = to_f32(in[t]);
-        const uint32_t w = seen[t - v0];
-        if (w) {
-            const uint32_t n = w & COUNT;
-            if (n || (w & IN_PROMPT)) x = x > 0.0f ? __fdiv_rn(x, rep) : x * rep;
-            if (n) x -= fmaf(freq, (float)n, pres);
-            if (w & HAS_BIAS) {
-                float b = 0.0f;
-                for (int i = 0; i < a.biases; ++i)
-                    if (ids[i] == t) b += values[i];
-                x += b;
-            }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int at = (j * THREADS + threadIdx.x) * NV, t = v0 + at;
+        if (t + NV <= 0 || t >= vocab) continue;
+        uint32_t allowed = ~0u;
+        if (mask) {  // NV bits from bit t on; bits in front of the row and behind it do not matter
+            const int first = t < 0 ? 0 : t, last = t + NV - 1 < vocab ? t + NV - 1 : vocab - 1;
+            const uint32_t lo = mask[first >> 5], hi = mask[last >> 5];
+            allowed = t < 0 ? lo << -t : __funnelshift_r(lo, hi, t & 31);
         }
-        if (mask && !((mask[t >> 5] >> (t & 31)) & 1)) x = -INFINITY;
-        out[t] = from_f32<T>(x);
+        uint32_t words[NV];
+#pragma unroll
+        for (int i = 0; i < NV / 4; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(&seen[at + 4 * i]);
+            words[4 * i] = w.x; words[4 * i + 1] = w.y; words[4 * i + 2] = w.z; words[4 * i + 3] = w.w;
+        }
+        float f[NV];
+        Pack<T>::unpack(x[j], f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (words[i]) f[i] = changed(f[i], words[i], rep, freq, pres, ids, values, a.biases, t + i);
+            if (!((allowed >> i) & 1)) f[i] = -INFINITY;
+        }
+        if (aligned_out && t >= 0 && t + NV <= vocab) {
+            *reinterpret_cast<uint4 *>(out + t) = Pack<T>::pack(f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (t + i >= 0 && t + i < vocab) out[t + i] = from_f32<T>(f[i]);
+        }
     }
 }
 
-template <typename T> int launch_logits(LogitsArgs a, int64_t rows, cudaStream_t st) {
+template <typename T, int VPT> void launch_tile(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
+    constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
+    // a skewed row may need one stretch more
+    launch_overlapped(logits_kernel<T, VPT>, dim3((unsigned)cdiv(a.vocab + NV - 1, TILE), (unsigned)rows), dim3(THREADS), 0, st, a);
+}
+
+template <typename T> int launch_logits(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
     note_indexed_launch();
-    a.tile = MAX_TILE;
-    launch_overlapped(logits_kernel<T>, dim3((unsigned)cdiv(a.vocab, a.tile), (unsigned)rows), dim3(THREADS), a.tile * sizeof(uint32_t), st, a);
+    constexpr int VPT = 8192 / THREADS / Pack<T>::N;
+    if (rows * cdiv(a.vocab, 8192) >= device_props().sm_count) launch_tile<T, VPT>(a, rows, st);
+    else launch_tile<T, VPT / 4>(a, rows, st);
     return check_launch("enc_penalize_logits");
 }
 
