@@ -26,9 +26,8 @@ struct LogitsArgs {
     int history, biases;
 };
 
-// The logit of a token that its count word says something about.  Not inlined: it is rare, and 32 copies of it in the
-// streaming loop outgrow the instruction cache (0.4 of all stalls at 256 x 131072).
-__device__ __noinline__ float changed(float x, uint32_t w, float rep, float freq, float pres, const int32_t *ids, const float *values, int biases, int t) {
+// The logit of a token that its count word says something about.
+__device__ __forceinline__ float changed(float x, uint32_t w, float rep, float freq, float pres, const int32_t *ids, const float *values, int biases, int t) {
     const uint32_t n = w & COUNT;
     if (n || (w & IN_PROMPT)) x = x > 0.0f ? __fdiv_rn(x, rep) : x * rep;
     if (n) x -= fmaf(freq, (float)n, pres);
@@ -44,9 +43,16 @@ __device__ __noinline__ float changed(float x, uint32_t w, float rep, float freq
 // VPT 16-byte vectors per thread: a stretch of VPT * THREADS vectors.  Stretches are cut so that the input's vectors are
 // aligned whatever the row's address: with `skew` elements of the row's first vector in front of the row, stretch i starts at
 // token i * TILE - skew.
-template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits_kernel(LogitsArgs a) {
+//
+// The tokens that something happens to are few but scattered: a warp streaming 32 vectors nearly always meets one, and the
+// whole warp would walk through the penalties for it, 900 instructions a warp at 256 x 131072.  So the thread that counts
+// a token first puts it on a list, the list is worked off with every lane busy, and the result goes back into the token's word
+// for the streaming loop to pick up.
+template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 4) logits_kernel(LogitsArgs a) {
     constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
-    __shared__ __align__(16) uint32_t seen[TILE];
+    extern __shared__ __align__(16) uint32_t seen[];  // [TILE] per token: what was counted, later ~(the bits of its new logit); 0: nothing
+    uint16_t *list = reinterpret_cast<uint16_t *>(seen + TILE);  // [TILE]
+    __shared__ int listed;
     const int64_t row = blockIdx.y;
     const T *in = reinterpret_cast<const T *>(a.in) + row * a.s_in;
     T *out = reinterpret_cast<T *>(a.out) + row * a.s_out;
@@ -72,6 +78,7 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits
     }
 #pragma unroll
     for (int i = 0; i < TILE / 4 / THREADS; ++i) reinterpret_cast<uint4 *>(seen)[i * THREADS + threadIdx.x] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) listed = 0;
     __syncthreads();
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     const bool reports = blockIdx.x == 0;  // one CTA per row reports what is out of range
@@ -86,8 +93,8 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits
         const int32_t *tok = a.tokens + row * a.s_tokens;
         auto count = [&](int t, int i) {
             if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
-                if (i < prompt) atomicOr(&seen[t - v0], IN_PROMPT);
-                else atomicAdd(&seen[t - v0], 1u);
+                const uint32_t before = i < prompt ? atomicOr(&seen[t - v0], IN_PROMPT) : atomicAdd(&seen[t - v0], 1u);
+                if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
             }
         };
         const int n4 = aligned16(tok) ? n / 4 : 0;
@@ -113,10 +120,19 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits
     const float *values = a.bias_values + row * a.s_bias;
     for (int i = threadIdx.x; i < a.biases; i += THREADS) {
         const int t = ids[i];
-        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) atomicOr(&seen[t - v0], HAS_BIAS);
-        else if (t < -1 || t >= vocab) bad = true;
+        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
+            if (atomicOr(&seen[t - v0], HAS_BIAS) == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
+        } else if (t < -1 || t >= vocab) {
+            bad = true;
+        }
     }
     if (bad && reports) atomicExch(&g_bad_index, 1u);
+    __syncthreads();
+    for (int i = threadIdx.x; i < listed; i += THREADS) {
+        const int at = list[i];
+        const float f = changed(to_f32(in[v0 + at]), seen[at], rep, freq, pres, ids, values, a.biases, v0 + at);
+        seen[at] = isnan(f) ? ~0x7fffffffu : ~__float_as_uint(f);  // (a NaN of all ones would read as nothing)
+    }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -138,7 +154,7 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits
         Pack<T>::unpack(x[j], f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (words[i]) f[i] = changed(f[i], words[i], rep, freq, pres, ids, values, a.biases, t + i);
+            if (words[i]) f[i] = __uint_as_float(~words[i]);
             if (!((allowed >> i) & 1)) f[i] = -INFINITY;
         }
         if (aligned_out && t >= 0 && t + NV <= vocab) {
@@ -153,8 +169,10 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS) logits
 
 template <typename T, int VPT> void launch_tile(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
     constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
+    constexpr int SMEM = TILE * 6;
+    cudaFuncSetAttribute(logits_kernel<T, VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     // a skewed row may need one stretch more
-    launch_overlapped(logits_kernel<T, VPT>, dim3((unsigned)cdiv(a.vocab + NV - 1, TILE), (unsigned)rows), dim3(THREADS), 0, st, a);
+    launch_overlapped(logits_kernel<T, VPT>, dim3((unsigned)cdiv(a.vocab + NV - 1, TILE), (unsigned)rows), dim3(THREADS), SMEM, st, a);
 }
 
 template <typename T> int launch_logits(const LogitsArgs &a, int64_t rows, cudaStream_t st) {

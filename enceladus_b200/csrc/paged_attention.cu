@@ -86,7 +86,7 @@ template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bound
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, sub = lane >> 3;
     const int D = a.head_dim;
     grid_dependency_wait();
-    walk_run<T, ROWS>(a, [&](int64_t seq, int kv_head, int first_head, int rows, int first, int keys, int t0, int t1, float *slot) {
+    walk_run<T, ROWS>(a, [&](int64_t seq, int kv_head, int first_head, int rows, int first, int skip, int keys, int t0, int t1, float *slot) {
         const T *qb = reinterpret_cast<const T *>(a.q) + seq * a.sq_s, *kb = reinterpret_cast<const T *>(a.k) + kv_head * a.sk_h;
         const T *vb = reinterpret_cast<const T *>(a.v) + kv_head * a.sv_h;
         float q[ROWS][CH][4], o[ROWS][CH][4], m[ROWS], l[ROWS];
@@ -110,7 +110,7 @@ template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bound
             const int j = j0 + sub;
             int64_t page = 0;
             int row = 0;
-            const bool in = j < stop && locate(a, seq, first + j, page, row);
+            const bool in = j < stop && j >= skip && locate(a, seq, first + j, page, row);
             float k[CH][4], v[CH][4];
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -313,6 +313,7 @@ extern "C" int enc_paged_attention(const enc_paged_cache *cache, const void *q, 
     a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.capacity = paged_capacity(*cache); a.window = window;
     a.q_heads = (int)q_heads; a.head_dim = (int)cache->head_dim; a.group = (int)(q_heads / cache->kv_heads);
     a.row_groups = p.row_groups; a.units = (int)cache->kv_heads * p.row_groups;
+    a.whole = cache->page_size % 16 == 0;
     a.min_run = 1;
     a.scale = sm_scale * LOG2E;
     a.page_size = FastDiv((uint32_t)cache->page_size);

@@ -37,6 +37,7 @@ struct PagedArgs {
     int64_t num_seqs, num_pages, capacity, window;
     int q_heads, head_dim, group, row_groups;  // query rows per kv head; row groups (of the kernel's row count) per kv head
     int units;                                 // row groups per sequence: kv_heads * row_groups
+    bool whole;                                // pages are whole multiples of 16 keys
     int min_run;                               // tiles a run has at least
     int merge_rows;                            // rows that a warp's part has in shared memory
     float scale;                               // sm_scale * log2(e)
@@ -44,14 +45,18 @@ struct PagedArgs {
 };
 
 // ---- schedule ------------------------------------------------------------------------------------
-// Keys of sequence b that its row looks at: the first key and how many.
-static __device__ __forceinline__ int keys_of(const PagedArgs &a, int64_t b, int &first) {
+// The keys that sequence b's row reads: `first` is the first one's position, the result how many.  Where pages are whole
+// multiples of 16 keys, `first` is rounded down to 16 and the `skip` (< 16) keys in front of the window are read but
+// not used.
+static __device__ __forceinline__ int keys_of(const PagedArgs &a, int64_t b, int &first, int &skip) {
     int n = a.seq_lens[b];
     if (n < 0 || n > a.capacity) {
         atomicExch(&g_bad_index, 1u);
         n = n < 0 ? 0 : (int)a.capacity;
     }
-    first = a.window > 0 && n > a.window ? n - (int)a.window : 0;
+    const int begin = a.window > 0 && n > a.window ? n - (int)a.window : 0;
+    first = a.whole ? begin & ~15 : begin;
+    skip = begin - first;
     return n - first;
 }
 static __device__ __forceinline__ int64_t tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
@@ -70,8 +75,8 @@ static __device__ __forceinline__ Run find_run(const PagedArgs &a) {
     const int64_t per = (a.num_seqs + THREADS - 1) / THREADS;
     const int64_t b0 = threadIdx.x * per, b1 = b0 + per < a.num_seqs ? b0 + per : a.num_seqs;
     int64_t mine = 0;
-    int first;
-    for (int64_t b = b0; b < b1; ++b) mine += tiles_of(keys_of(a, b, first));
+    int first, skip;
+    for (int64_t b = b0; b < b1; ++b) mine += tiles_of(keys_of(a, b, first, skip));
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -97,7 +102,7 @@ static __device__ __forceinline__ Run find_run(const PagedArgs &a) {
     if (before * a.units <= r.begin && r.begin < (before + mine) * a.units) {
         int64_t at = r.begin - before * a.units;
         for (int64_t b = b0; b < b1; ++b) {
-            const int64_t t = tiles_of(keys_of(a, b, first)) * a.units;
+            const int64_t t = tiles_of(keys_of(a, b, first, skip)) * a.units;
             if (at < t) {
                 found[0] = b;
                 found[1] = at;
@@ -152,8 +157,8 @@ static __device__ __forceinline__ void write_piece(const PagedArgs &a, const flo
 template <typename T> __device__ __forceinline__ void write_empty_rows(const PagedArgs &a) {
     T *o = reinterpret_cast<T *>(a.o);
     for (int64_t b = blockIdx.x; b < a.num_seqs; b += gridDim.x) {  // rows without keys
-        int first;
-        if (keys_of(a, b, first) > 0) continue;
+        int first, skip;
+        if (keys_of(a, b, first, skip) > 0) continue;
         for (int i = threadIdx.x; i < a.q_heads * a.head_dim; i += THREADS) {
             const int h = i / a.head_dim, d = i - h * a.head_dim;
             o[b * a.so_s + h * a.so_h + d] = from_f32<T>(0.0f);
@@ -162,15 +167,15 @@ template <typename T> __device__ __forceinline__ void write_empty_rows(const Pag
     }
 }
 
-// Walks over the CTA's run: process(seq, kv head, first query head, rows, first key, keys, tile range, slot or NULL) per
+// Walks over the CTA's run: process(seq, kv head, first query head, rows, first key, keys to skip, keys, tile range, slot or NULL) per
 // piece.  Also writes the header that the join reads, and the rows of sequences without keys.
 template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk_run(const PagedArgs &a, F process) {
     const Run run = find_run(a);
     if (threadIdx.x == 0 && a.headers) a.headers[blockIdx.x].y = 0;
     int64_t seq = run.seq, at = run.at;
     for (int64_t pos = run.begin; pos < run.end;) {
-        int first;
-        const int keys = keys_of(a, seq, first);
+        int first, skip;
+        const int keys = keys_of(a, seq, first, skip);
         const int64_t tiles = tiles_of(keys);
         if (at >= tiles * a.units) {
             at -= tiles * a.units;  // (zero: a sequence's tiles are walked to their end)
@@ -189,7 +194,7 @@ template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk
             slot = slot_of(a, blockIdx.x, 1, ROWS);
             if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), (int)((pos + tiles - 1) / run.run), 0);
         }
-        process(seq, kv_head, first_head, rows, first, keys, t0, t1, slot);
+        process(seq, kv_head, first_head, rows, first, skip, keys, t0, t1, slot);
         pos += t1 - t0;
         at += t1 - t0;
     }

@@ -48,13 +48,13 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { retu
 // A place in the CTA's run: a tile of one unit (kv head and row group) of one sequence.
 struct Cursor {
     int64_t left, seq;  // tiles left in the run
-    int unit, t, tiles, keys, first;
+    int unit, t, tiles, keys, first, skip;
 
     __device__ __forceinline__ void start(const PagedArgs &a, const Run &run) {
         left = run.end - run.begin;
         if (left <= 0) return;
         seq = run.seq;
-        keys = keys_of(a, seq, first);
+        keys = keys_of(a, seq, first, skip);
         tiles = (int)tiles_of(keys);
         unit = (int)(run.at / tiles);
         t = (int)(run.at - (int64_t)unit * tiles);
@@ -67,13 +67,13 @@ struct Cursor {
         unit = 0;
         do {  // (left > 0: a sequence with keys follows)
             ++seq;
-            keys = keys_of(a, seq, first);
+            keys = keys_of(a, seq, first, skip);
         } while (keys == 0);
         tiles = (int)tiles_of(keys);
     }
 };
 
-template <typename T, int D, int STAGES, int CTAS> __global__ void __launch_bounds__(THREADS, CTAS) paged_mma_kernel(PagedArgs a) {
+template <typename T, int D, int STAGES, int CTAS, bool WHOLE> __global__ void __launch_bounds__(THREADS, CTAS) paged_mma_kernel(PagedArgs a) {
     using R = Ring<D, STAGES>;
     constexpr int KS = D / 16, CHUNKS = D / 8;  // steps of the first product; 16-byte chunks of a row
     constexpr float LOWER = std::is_same<T, __half>::value ? 14.0f : 0.0f;
@@ -90,33 +90,60 @@ template <typename T, int D, int STAGES, int CTAS> __global__ void __launch_boun
     Cursor load, at;
     load.start(a, run);
     at = load;
-    int page = 0;  // of this lane's key in the tile that is loaded next: read one tile ahead
+    // Page number that the next copies need, read one tile ahead.  WHOLE: pages are whole multiples of 16 keys and so is the
+    // first key, so a warp's 16 keys lie in one page and their rows at one distance; otherwise every lane looks up its key.
+    int page = 0;
     auto read_page = [&]() {
         if (load.left <= 0) return;
-        const int j = load.t * TILE + warp * 16 + (lane & 15);
+        const int j = load.t * TILE + warp * 16 + (WHOLE ? 0 : lane & 15);
         if (j < load.keys) page = a.block_table[load.seq * a.s_table + a.page_size.div((uint32_t)(load.first + j))];
     };
     auto issue = [&](int stage) {  // the copies of one tile's 16 keys and values, then one step on
         if (load.left > 0) {
-            const int j = load.t * TILE + warp * 16 + (lane & 15);
+            const int j0 = load.t * TILE + warp * 16, n = load.keys - j0;  // keys of the 16 that exist
             const int kv_head = a.row_groups == 1 ? load.unit : load.unit / a.row_groups;
-            const T *row = nullptr;  // lanes 0-15: the key rows; 16-31: the value rows
-            if (j < load.keys) {
-                const uint32_t pos = (uint32_t)(load.first + j);
-                const int in_page = (int)(pos - a.page_size.div(pos) * a.page_size.d);
-                if (page >= 0 && page < a.num_pages)
-                    row = lane < 16 ? reinterpret_cast<const T *>(a.k) + page * a.sk_p + kv_head * a.sk_h + in_page * a.sk_t
-                                    : reinterpret_cast<const T *>(a.v) + page * a.sv_p + kv_head * a.sv_h + in_page * a.sv_t;
-                else atomicExch(&g_bad_index, 1u);
-            }
+            const T *kb = reinterpret_cast<const T *>(a.k) + kv_head * a.sk_h, *vb = reinterpret_cast<const T *>(a.v) + kv_head * a.sv_h;
             const uint32_t dst = ring + stage * 2 * R::HALF;
+            const bool ok = page >= 0 && page < a.num_pages;
+            const uint32_t pos = (uint32_t)(load.first + j0 + (WHOLE ? 0 : lane & 15));
+            const int in_page = (int)(pos - a.page_size.div(pos) * a.page_size.d);
+            if (n > 0 && !ok && (WHOLE ? lane == 0 : (lane & 15) < n)) atomicExch(&g_bad_index, 1u);
+            const int skip = WHOLE && load.t == 0 && warp == 0 ? load.skip : 0;
+            if (WHOLE && n >= 16 && skip == 0 && ok) {  // all of a page's 16 keys: no tests
+                const T *k = kb + page * a.sk_p + in_page * a.sk_t, *v = vb + page * a.sv_p + in_page * a.sv_t;
+                if constexpr (32 % CHUNKS == 0) {  // the same place of the row in every step: one pointer each, moved on
+                    constexpr int ROWS_A_STEP = 32 / CHUNKS;
+                    const T *kp = k + (lane / CHUNKS) * a.sk_t + lane % CHUNKS * 8, *vp = v + (lane / CHUNKS) * a.sv_t + lane % CHUNKS * 8;
+                    const uint32_t to = dst + lane / CHUNKS * R::PITCH + lane % CHUNKS * 16;
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const int idx = i * 32 + lane, r = idx / CHUNKS, c = idx - r * CHUNKS;
-                const T *k = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r));
-                const T *v = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), 16 + r));
-                cp_async16(dst + r * R::PITCH + c * 16, k ? k + c * 8 : reinterpret_cast<const T *>(a.k), k ? 16 : 0);
-                cp_async16(dst + R::HALF + r * R::PITCH + c * 16, v ? v + c * 8 : reinterpret_cast<const T *>(a.v), v ? 16 : 0);
+                    for (int i = 0; i < KS; ++i) {
+                        cp_async16(to + i * ROWS_A_STEP * R::PITCH, kp);
+                        cp_async16(to + i * ROWS_A_STEP * R::PITCH + R::HALF, vp);
+                        kp += ROWS_A_STEP * a.sk_t;
+                        vp += ROWS_A_STEP * a.sv_t;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        const int idx = i * 32 + lane, r = idx / CHUNKS, c = idx - r * CHUNKS;
+                        cp_async16(dst + r * R::PITCH + c * 16, k + (r * a.sk_t + c * 8));
+                        cp_async16(dst + R::HALF + r * R::PITCH + c * 16, v + (r * a.sv_t + c * 8));
+                    }
+                }
+            } else if (n > 0) {
+                const T *row = nullptr;  // of key lane & 15; lanes 0-15: the key rows, 16-31: the value rows
+                if (ok && (lane & 15) < n && (lane & 15) >= skip) {
+                    const int64_t at = in_page + (WHOLE ? lane & 15 : 0);
+                    row = lane < 16 ? kb + page * a.sk_p + at * a.sk_t : vb + page * a.sv_p + at * a.sv_t;
+                }
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const int idx = i * 32 + lane, r = idx / CHUNKS, c = idx - r * CHUNKS;
+                    const T *k = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r));
+                    const T *v = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), 16 + r));
+                    cp_async16(dst + r * R::PITCH + c * 16, k ? k + c * 8 : reinterpret_cast<const T *>(a.k), k ? 16 : 0);
+                    cp_async16(dst + R::HALF + r * R::PITCH + c * 16, v ? v + c * 8 : reinterpret_cast<const T *>(a.v), v ? 16 : 0);
+                }
             }
             load.next(a);
             read_page();
@@ -175,40 +202,52 @@ template <typename T, int D, int STAGES, int CTAS> __global__ void __launch_boun
                 mma16816<T>(s[1], q[i], b[2], b[3]);
             }
             uint32_t hi[4], lo[4];  // P as the left operand of the second product
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                s[0][x] *= a.scale;
+                s[1][x] *= a.scale;
+            }
+            if (left < 16) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    if ((x >> 2) * 8 + qc + (x & 1) >= left) s[x >> 2][x & 3] = -INFINITY;
+            }
+            if (at.skip > 0 && at.t == 0 && warp == 0) {  // keys in front of the window
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    if ((x >> 2) * 8 + qc + (x & 1) < at.skip) s[x >> 2][x & 3] = -INFINITY;
+            }
             bool grew = false;
-            float up[2], base[2];
+            float up[2] = {1.0f, 1.0f}, base[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float &x = s[n][2 * h + e];
-                        x = n * 8 + qc + e < left ? x * a.scale : -INFINITY;
-                        top = fmaxf(top, x);
-                    }
+                if (h == 1 && rows <= 8) continue;  // the lower eight rows hold no queries
+                float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - LOWER;
-                up[h] = 1.0f;
                 if (top > m[h]) {
                     up[h] = m[h] == -INFINITY ? 0.0f : fast_exp2(m[h] - top);
                     m[h] = top;
                     grew = true;
                 }
                 base[h] = m[h] == -INFINITY ? 0.0f : m[h];
-                l[h] *= up[h];
             }
             if (__any_sync(0xffffffffu, grew)) {  // rare after the first keys of a row
+#pragma unroll
+                for (int h = 0; h < 2; ++h) l[h] *= up[h];
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) o[i][x] *= up[x >> 1];
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && rows <= 8) {
+                    hi[1] = hi[3] = lo[1] = lo[3] = 0;
+                    continue;
+                }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int n = 0; n < 2; ++n) {
                     const float p0 = fast_exp2(s[n][2 * h] - base[h]), p1 = fast_exp2(s[n][2 * h + 1] - base[h]);
                     l[h] += p0 + p1;
                     const uint32_t x = pack2<T>(p0, p1);
@@ -216,6 +255,7 @@ template <typename T, int D, int STAGES, int CTAS> __global__ void __launch_boun
                     hi[2 * n + h] = x;
                     lo[2 * n + h] = pack2<T>(p0 - r.x, p1 - r.y);
                 }
+            }
             const uint32_t vaddr = vs + (lane & 15) * R::PITCH + (lane >> 4) * 16;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
@@ -269,7 +309,7 @@ template <typename T, int D, int STAGES, int CTAS> __global__ void __launch_boun
 
 template <typename T, int D, int STAGES, int CTAS> int launch(PagedArgs a, int grid, cudaStream_t st) {
     using R = Ring<D, STAGES>;
-    auto kern = paged_mma_kernel<T, D, STAGES, CTAS>;
+    auto kern = a.whole ? paged_mma_kernel<T, D, STAGES, CTAS, true> : paged_mma_kernel<T, D, STAGES, CTAS, false>;
     a.merge_rows = a.group < MMA_ROWS ? a.group : MMA_ROWS;
     const int smem = R::TOTAL + WARPS * a.merge_rows * R::O_STRIDE * 4;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
