@@ -13,7 +13,7 @@
 namespace enc {
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 512;
 constexpr uint32_t IN_PROMPT = 1u << 31, HAS_BIAS = 1u << 30;          // above the count, which the history's length bounds
 constexpr uint32_t COUNT = HAS_BIAS - 1;
 
@@ -48,7 +48,7 @@ __device__ __forceinline__ float changed(float x, uint32_t w, float rep, float f
 // whole warp would walk through the penalties for it, 900 instructions a warp at 256 x 131072.  So the thread that counts
 // a token first puts it on a list, the list is worked off with every lane busy, and the result goes back into the token's word
 // for the streaming loop to pick up.
-template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 4) logits_kernel(LogitsArgs a) {
+template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) logits_kernel(LogitsArgs a) {
     constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
     extern __shared__ __align__(16) uint32_t seen[];  // [TILE] per token: what was counted, later ~(the bits of its new logit); 0: nothing
     uint16_t *list = reinterpret_cast<uint16_t *>(seen + TILE);  // [TILE]
@@ -63,7 +63,24 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 4) log
     const bool aligned_out = reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == skew;
     const int32_t *mask = a.mask ? a.mask + row * a.s_mask : nullptr;
     grid_dependency_wait();
-    // the logits are on their way while the history is counted
+    // Everything that the counting needs and the logits themselves are asked for at once: a stretch takes a few microseconds,
+    // and one round trip to memory after the other would be most of them.
+    constexpr int UN = 4;  // vectors of the history in flight per thread
+    const int32_t *tok = a.tokens + row * a.s_tokens;
+    const int history = a.tokens ? a.history : 0, h4 = aligned16(tok) ? history / 4 : 0;
+    const int4 nothing = make_int4(-1, -1, -1, -1);
+    int4 token[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) token[u] = (int)threadIdx.x + u * THREADS < h4 ? reinterpret_cast<const int4 *>(tok)[threadIdx.x + u * THREADS] : nothing;
+    int n = 0, prompt = 0;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (a.tokens) {
+        n = a.lens[row];
+        prompt = a.prompt_lens[row];
+        rep = a.repetition[row];
+        freq = a.frequency[row];
+        pres = a.presence[row];
+    }
     uint4 x[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -80,42 +97,34 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 4) log
     for (int i = 0; i < TILE / 4 / THREADS; ++i) reinterpret_cast<uint4 *>(seen)[i * THREADS + threadIdx.x] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     const bool reports = blockIdx.x == 0;  // one CTA per row reports what is out of range
-    bool bad = false;
-    if (a.tokens) {
-        int n = a.lens[row], prompt = a.prompt_lens[row];
-        bad = n < 0 || n > a.history || prompt < 0 || prompt > n;
-        n = n < 0 ? 0 : n > a.history ? a.history : n;
-        rep = a.repetition[row];
-        freq = a.frequency[row];
-        pres = a.presence[row];
-        const int32_t *tok = a.tokens + row * a.s_tokens;
-        auto count = [&](int t, int i) {
-            if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
-                const uint32_t before = i < prompt ? atomicOr(&seen[t - v0], IN_PROMPT) : atomicAdd(&seen[t - v0], 1u);
-                if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
-            }
-        };
-        const int n4 = aligned16(tok) ? n / 4 : 0;
-        constexpr int UN = 4;  // vectors in flight per thread
-        for (int i = threadIdx.x; i < n4; i += UN * THREADS) {
-            int4 t[UN];
-#pragma unroll
-            for (int u = 0; u < UN; ++u) t[u] = i + u * THREADS < n4 ? reinterpret_cast<const int4 *>(tok)[i + u * THREADS] : make_int4(-1, -1, -1, -1);
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const int at = 4 * (i + u * THREADS);
-                count(t[u].x, at);
-                count(t[u].y, at + 1);
-                count(t[u].z, at + 2);
-                count(t[u].w, at + 3);
-            }
+    bool bad = n < 0 || n > history || prompt < 0 || prompt > n;
+    n = n < 0 ? 0 : n > history ? history : n;
+    auto count = [&](int t, int i) {
+        if (i >= n) return;
+        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
+            const uint32_t before = i < prompt ? atomicOr(&seen[t - v0], IN_PROMPT) : atomicAdd(&seen[t - v0], 1u);
+            if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
+        } else if (reports) {
+            bad |= (unsigned)t >= (unsigned)vocab;
         }
-        for (int i = 4 * n4 + threadIdx.x; i < n; i += THREADS) count(tok[i], i);
-        if (reports)
-            for (int i = threadIdx.x; i < n; i += THREADS) bad |= (unsigned)tok[i] >= (unsigned)vocab;
+    };
+    for (int i = threadIdx.x; i < h4 && 4 * i < n; i += UN * THREADS) {
+        if (i >= UN * THREADS) {
+#pragma unroll
+            for (int u = 0; u < UN; ++u) token[u] = i + u * THREADS < h4 ? reinterpret_cast<const int4 *>(tok)[i + u * THREADS] : nothing;
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int at = 4 * (i + u * THREADS);
+            if (at >= n) break;
+            count(token[u].x, at);
+            count(token[u].y, at + 1);
+            count(token[u].z, at + 2);
+            count(token[u].w, at + 3);
+        }
     }
+    for (int i = 4 * h4 + threadIdx.x; i < n; i += THREADS) count(tok[i], i);
     const int32_t *ids = a.bias_ids + row * a.s_bias;
     const float *values = a.bias_values + row * a.s_bias;
     for (int i = threadIdx.x; i < a.biases; i += THREADS) {
@@ -179,7 +188,7 @@ template <typename T> int launch_logits(const LogitsArgs &a, int64_t rows, cudaS
     note_indexed_launch();
     constexpr int VPT = 8192 / THREADS / Pack<T>::N;
     if (rows * cdiv(a.vocab, 8192) >= device_props().sm_count) launch_tile<T, VPT>(a, rows, st);
-    else launch_tile<T, VPT / 4>(a, rows, st);
+    else launch_tile<T, 1>(a, rows, st);
     return check_launch("enc_penalize_logits");
 }
 

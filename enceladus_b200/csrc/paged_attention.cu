@@ -175,7 +175,7 @@ template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bound
                 }
         }
         __syncthreads();
-        write_piece<T, ROWS>(a, so, ROWS * MAX_HEAD_DIM, MAX_HEAD_DIM, sm, sl, rows, seq, first_head, slot);
+        write_piece<T, ROWS>(a, so, ROWS * MAX_HEAD_DIM, MAX_HEAD_DIM, sm, sl, rows, seq, first_head, slot, 0, D);
         __syncthreads();
     });
 }
@@ -200,7 +200,7 @@ struct Plan {
 void make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant, Plan &p) {
     const int group = (int)(q_heads / c.kv_heads);
     p.variant = variant >= 0 ? variant : tensor_ok(c, dtype) ? V_TENSOR : V_CORES;
-    p.rows = p.variant == V_TENSOR ? MMA_ROWS : group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
+    p.rows = p.variant == V_TENSOR ? mma_rows(group) : group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
     const int per_sm = p.variant == V_TENSOR ? mma_ctas_per_sm(c.head_dim) : 4;
     p.row_groups = (int)cdiv(group, p.rows);
     const int64_t most = c.num_seqs * c.kv_heads * p.row_groups * cdiv(paged_capacity(c), TILE);  // tiles if every row is full
@@ -228,7 +228,8 @@ template <typename T> int launch_paged(const PagedArgs &a, const Plan &p, cudaSt
         if (p.variant == V_TENSOR) {
             const int rc = launch_mma(a, std::is_same<T, __half>::value ? ENC_F16 : ENC_BF16, p.grid, st);
             if (rc != ENC_OK) return rc;
-            launch_join<T, MMA_ROWS>(a, p.grid, st);
+            if (p.rows == 8) launch_join<T, 8>(a, p.grid, st);
+            else launch_join<T, 16>(a, p.grid, st);
             return check_launch("enc_paged_attention");
         }
     }
@@ -269,7 +270,7 @@ unsigned int take_bad_index_paged_mma();
 unsigned int take_bad_index_paged_attention() { return take_bad_index_word() | take_bad_index_paged_mma(); }
 int paged_attention_variants() { return VARIANTS; }
 void paged_attention_variant_info(int v, char *out, size_t n) {
-    if (v == V_TENSOR) snprintf(out, n, "mma m16n8k16, 16 query rows, 16 keys per warp and step, keys and values through a cp.async ring");
+    if (v == V_TENSOR) snprintf(out, n, "mma m16n8k16, 16 keys by 8 or 16 query rows per warp and step, keys and values through a cp.async ring");
     else snprintf(out, n, "CUDA cores, eight lanes per key, keys and values straight to registers");
 }
 

@@ -39,7 +39,8 @@ struct PagedArgs {
     int units;                                 // row groups per sequence: kv_heads * row_groups
     bool whole;                                // pages are whole multiples of 16 keys
     int min_run;                               // tiles a run has at least
-    int merge_rows;                            // rows that a warp's part has in shared memory
+    bool q_pairs;                              // query elements can be read two at a time
+    int merge_rows, merge_dims;                // rows and elements of a warp's part that shared memory holds at a time
     float scale;                               // sm_scale * log2(e)
     FastDiv page_size;
 };
@@ -122,13 +123,13 @@ static __device__ __forceinline__ float *slot_of(const PagedArgs &a, int64_t cta
 }
 
 // A piece's rows, one partial result per warp in shared memory (O unnormalised, rows `stride` apart, m and l),
-// joined and written: to the output when the piece is the whole row, to `slot` otherwise.
+// joined and written (elements d0 .. d0 + dims - 1 of the head, `so` starting at d0): to the output when the piece is the whole row, to `slot` otherwise.
 template <typename T, int ROWS>
 static __device__ __forceinline__ void write_piece(const PagedArgs &a, const float *so, int warp_stride, int stride, const float (*sm)[ROWS], const float (*sl)[ROWS],
-                                            int rows, int64_t seq, int first_head, float *slot) {
+                                            int rows, int64_t seq, int first_head, float *slot, int d0, int dims) {
     T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s;
-    for (int i = threadIdx.x; i < rows * a.head_dim; i += THREADS) {
-        const int r = i / a.head_dim, d = i - r * a.head_dim;
+    for (int i = threadIdx.x; i < rows * dims; i += THREADS) {
+        const int r = i / dims, e = i - r * dims, d = d0 + e;
         float m = sm[0][r];
 #pragma unroll
         for (int w = 1; w < WARPS; ++w) m = fmaxf(m, sm[w][r]);
@@ -138,7 +139,7 @@ static __device__ __forceinline__ void write_piece(const PagedArgs &a, const flo
         for (int w = 0; w < WARPS; ++w) {
             const float c = fast_exp2(sm[w][r] - base);
             l = fmaf(sl[w][r], c, l);
-            x = fmaf(so[w * warp_stride + r * stride + d], c, x);
+            x = fmaf(so[w * warp_stride + r * stride + e], c, x);
         }
         if (slot) {
             slot[r * (a.head_dim + 2) + d] = x;
@@ -213,8 +214,8 @@ static __device__ __forceinline__ bool locate(const PagedArgs &a, int64_t seq, i
 
 
 // Tensor-core kernels (paged_attention_mma.cu): whether there is one for this head_dim, CTAs per SM, and the launch.
-int mma_ctas_per_sm(int64_t head_dim);  // 0: none
-constexpr int MMA_ROWS = 16;
+int mma_ctas_per_sm(int64_t head_dim);                       // 0: none
+inline int mma_rows(int group) { return group <= 8 ? 8 : 16; }  // query rows that a CTA takes at a time
 int launch_mma(const PagedArgs &a, int dtype, int grid, cudaStream_t st);
 
 }  // namespace paged

@@ -1,19 +1,26 @@
 // Attention of one new token per sequence over a paged key-value cache: the tensor-core kernel for 16-bit types.
 // Mathematics, bound and split are in paged_attention.cuh.
 //
-// The up to 16 query heads that share a kv head are the rows of an m16n8k16 product: S = Q K^T over 16 keys per warp and step,
-// O += P V with P taken from S's registers.  The unit is bound by HBM, so the tensor pipe's rate does not matter (at 6.5 TB/s
-// an SM has about 350 cycles for 16 keys of 128 elements, and spends 48 of these instructions on them); what the matrix
-// instruction buys is that the work per key no longer grows with the number of query heads.  tcgen05 would need 128 query rows
-// to fill its smallest tile, and its operands would still come through shared memory.
+// The query heads that share a kv head are the columns of an m16n8k16 product: S^T = K Q^T over 16 keys per warp and step, and
+// O^T += V^T P^T over the same 16 keys, 8 heads at a time (two columns blocks for 9 to 16).  With the keys as rows nothing is
+// padded up to 16 but the keys themselves: against queries as rows the matrix instructions and the registers of O and Q
+// halve for groups of up to 8 heads.  P^T needs the layout of S^T transposed: one movmatrix per 8 x 8 block.
+//
+// The kernel is bound by HBM as long as a warp's step (about 250 instructions on 8 KB) stays short; the tensor pipe's rate does
+// not matter.  What the matrix instruction buys is that the work per key hardly grows with the number of query heads.
+// tcgen05 would need 128 rows of keys or queries to fill its smallest tile.
 //
 // Each warp has a ring of its own in shared memory and walks its keys without CTA barriers: 16 keys and 16 values per stage,
 // 16-byte asynchronous copies, rows padded by 16 bytes so that ldmatrix meets no bank twice.  The ring runs on across the
 // pieces of a run: the next row's keys are on their way while a finished one is joined and written.
 //
 // P is fed as the sum of two 16-bit numbers, P = hi + lo, in two products: the weights keep 16 or more bits instead of 8 or 11
-// and the output is as exact as a float32 product rounded once.  In fp16 the maximum is kept 14 powers of two lower, so that
-// weights down to 2^-28 of the largest are still normal numbers.
+// and the output is as exact as a float32 product rounded once.
+//
+// The maximum that weights are taken relative to moves only when a score passes it by SLACK powers of two, so nearly all
+// steps need neither the reduction over the keys nor the rescaling; l and O use the same reference, so the result is the
+// same.  In fp16 the reference is kept 14 powers of two below the maximum it was taken from, so that weights down to 2^-28 of
+// the largest are normal numbers, and it moves as soon as a weight would pass 2^15.
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -27,8 +34,10 @@ template <int D, int STAGES> struct Ring {
     static constexpr int HALF = 16 * PITCH;              // 16 keys (or values)
     static constexpr int WARP = STAGES * 2 * HALF;
     static constexpr int TOTAL = WARPS * WARP;
-    static constexpr int O_STRIDE = D + 8;               // floats of a row of partial results
 };
+// Floats of a row of partial results: 4 more than a multiple of 16, so that the 8 elements x 4 row pairs that a warp writes
+// at a time meet 32 banks.
+__host__ __device__ constexpr int part_stride(int dims) { return dims + 4; }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
@@ -73,16 +82,17 @@ struct Cursor {
     }
 };
 
-template <typename T, int D, int STAGES, int CTAS, bool WHOLE> __global__ void __launch_bounds__(THREADS, CTAS) paged_mma_kernel(PagedArgs a) {
+template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global__ void __launch_bounds__(THREADS, CTAS) paged_mma_kernel(PagedArgs a) {
     using R = Ring<D, STAGES>;
     constexpr int KS = D / 16, CHUNKS = D / 8;  // steps of the first product; 16-byte chunks of a row
-    constexpr float LOWER = std::is_same<T, __half>::value ? 14.0f : 0.0f;
+    constexpr int ROWS = 8 * NQ;
+    constexpr float LOWER = std::is_same<T, __half>::value ? 14.0f : 0.0f, SLACK = std::is_same<T, __half>::value ? 15.0f : 16.0f;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float sm[WARPS][MMA_ROWS], sl[WARPS][MMA_ROWS];
+    __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS];
     float *so = reinterpret_cast<float *>(smem + R::TOTAL);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t ring = smem_addr(smem) + warp * R::WARP;
-    const int qr = lane >> 2, qc = (lane & 3) * 2;  // this thread's row (and row + 8) and first column in accumulators
+    const int lr = lane >> 2, lc = (lane & 3) * 2;  // this thread's row (and row + 8) and first column in accumulators
     grid_dependency_wait();
     const Run run = find_run(a);
     if (threadIdx.x == 0 && a.headers) a.headers[blockIdx.x].y = 0;
@@ -154,8 +164,8 @@ template <typename T, int D, int STAGES, int CTAS, bool WHOLE> __global__ void _
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) issue(s);
 
-    uint32_t q[KS][4];
-    float o[D / 8][4], m[2], l[2];
+    uint32_t q[KS][NQ][2];
+    float o[KS][NQ][4], m[NQ][2], l[NQ][2];  // O^T: rows i * 16 + lr (+ 8) of the head, columns lc, lc + 1 of the query block
     bool fresh = true;
     int64_t seq = 0;
     int first_head = 0, rows = 0, t0 = 0, stage = 0;
@@ -165,106 +175,117 @@ template <typename T, int D, int STAGES, int CTAS, bool WHOLE> __global__ void _
             seq = at.seq;
             t0 = at.t;
             const int kv_head = a.row_groups == 1 ? at.unit : at.unit / a.row_groups, rg = at.unit - kv_head * a.row_groups;
-            rows = a.group - rg * MMA_ROWS < MMA_ROWS ? a.group - rg * MMA_ROWS : MMA_ROWS;
-            first_head = kv_head * a.group + rg * MMA_ROWS;
+            rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
+            first_head = kv_head * a.group + rg * ROWS;
             const T *qp = reinterpret_cast<const T *>(a.q) + seq * a.sq_s + (int64_t)first_head * a.sq_h;
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
+            for (int b = 0; b < NQ; ++b) {
+                const T *p = qp + (b * 8 + lr) * a.sq_h + lc;
+                const bool there = b * 8 + lr < rows;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int r = qr + (x & 1) * 8, d = i * 16 + (x >> 1) * 8 + qc;
+                for (int i = 0; i < 2 * KS; ++i) {
                     uint32_t v = 0;
-                    if (r < rows) {
-                        const T *p = qp + r * a.sq_h + d;
-                        v = (uint32_t)*reinterpret_cast<const uint16_t *>(p) | (uint32_t)*reinterpret_cast<const uint16_t *>(p + 1) << 16;
-                    }
-                    q[i][x] = v;
+                    if (there && a.q_pairs) v = *reinterpret_cast<const uint32_t *>(p + i * 8);
+                    else if (there) v = (uint32_t)*reinterpret_cast<const uint16_t *>(p + i * 8) | (uint32_t)*reinterpret_cast<const uint16_t *>(p + i * 8 + 1) << 16;
+                    q[i / 2][b][i % 2] = v;
                 }
-            m[0] = m[1] = -INFINITY;
-            l[0] = l[1] = 0.0f;
+                m[b][0] = m[b][1] = -INFINITY;
+                l[b][0] = l[b][1] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i)
+                for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[i][x] = 0.0f;
+                    for (int x = 0; x < 4; ++x) o[i][b][x] = 0.0f;
+            }
         }
         cp_async_wait<STAGES - 1>();
         __syncwarp();
         const int left = at.keys - (at.t * TILE + warp * 16);  // keys of this warp's 16 that exist
         if (left > 0) {
             const uint32_t ks = ring + stage * 2 * R::HALF, vs = ks + R::HALF;
-            float s[2][4] = {};
-            const uint32_t kaddr = ks + ((lane & 7) + (lane >> 4) * 8) * R::PITCH + ((lane >> 3) & 1) * 16;
+            float s[NQ][4];
+            {
+                float odd[NQ][4] = {};  // two chains of products, added at the end
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                uint32_t b[4];
-                ldsm4(b, kaddr + i * 32);
-                mma16816<T>(s[0], q[i], b[0], b[1]);
-                mma16816<T>(s[1], q[i], b[2], b[3]);
-            }
-            uint32_t hi[4], lo[4];  // P as the left operand of the second product
+                for (int b = 0; b < NQ; ++b)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                s[0][x] *= a.scale;
-                s[1][x] *= a.scale;
+                    for (int x = 0; x < 4; ++x) s[b][x] = 0.0f;
+                const uint32_t kaddr = ks + (lane & 15) * R::PITCH + (lane >> 4) * 16;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t k[4];
+                    ldsm4(k, kaddr + i * 32);
+#pragma unroll
+                    for (int b = 0; b < NQ; ++b) mma16816<T>(i & 1 ? odd[b] : s[b], k, q[i][b][0], q[i][b][1]);
+                }
+#pragma unroll
+                for (int b = 0; b < NQ; ++b)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[b][x] = (s[b][x] + odd[b][x]) * a.scale;
             }
             if (left < 16) {
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    if ((x >> 2) * 8 + qc + (x & 1) >= left) s[x >> 2][x & 3] = -INFINITY;
-            }
-            if (at.skip > 0 && at.t == 0 && warp == 0) {  // keys in front of the window
+                for (int b = 0; b < NQ; ++b)
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    if ((x >> 2) * 8 + qc + (x & 1) < at.skip) s[x >> 2][x & 3] = -INFINITY;
+                    for (int x = 0; x < 4; ++x)
+                        if (lr + (x >> 1) * 8 >= left) s[b][x] = -INFINITY;
             }
-            bool grew = false;
-            float up[2] = {1.0f, 1.0f}, base[2];
+            if (WHOLE && at.skip > 0 && at.t == 0 && warp == 0) {  // keys in front of the window
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h == 1 && rows <= 8) continue;  // the lower eight rows hold no queries
-                float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - LOWER;
-                if (top > m[h]) {
-                    up[h] = m[h] == -INFINITY ? 0.0f : fast_exp2(m[h] - top);
-                    m[h] = top;
-                    grew = true;
+                for (int b = 0; b < NQ; ++b)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (lr + (x >> 1) * 8 < at.skip) s[b][x] = -INFINITY;
+            }
+            bool over = false;
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) over |= fmaxf(s[b][0], s[b][2]) > m[b][0] + SLACK || fmaxf(s[b][1], s[b][3]) > m[b][1] + SLACK;
+            if (__any_sync(0xffffffffu, over)) {  // rare after the first keys of a row
+#pragma unroll
+                for (int b = 0; b < NQ; ++b) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float top = fmaxf(s[b][c], s[b][c + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - LOWER;
+                        if (top > m[b][c]) {
+                            const float down = m[b][c] == -INFINITY ? 0.0f : fast_exp2(m[b][c] - top);
+                            m[b][c] = top;
+                            l[b][c] *= down;
+#pragma unroll
+                            for (int i = 0; i < KS; ++i) {
+                                o[i][b][c] *= down;
+                                o[i][b][c + 2] *= down;
+                            }
+                        }
+                    }
                 }
-                base[h] = m[h] == -INFINITY ? 0.0f : m[h];
             }
-            if (__any_sync(0xffffffffu, grew)) {  // rare after the first keys of a row
+            uint32_t hi[NQ][2], lo[NQ][2];  // P^T as the right operand of the second product
 #pragma unroll
-                for (int h = 0; h < 2; ++h) l[h] *= up[h];
+            for (int b = 0; b < NQ; ++b) {
+                const float base0 = m[b][0] == -INFINITY ? 0.0f : m[b][0], base1 = m[b][1] == -INFINITY ? 0.0f : m[b][1];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) o[i][x] *= up[x >> 1];
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h == 1 && rows <= 8) {
-                    hi[1] = hi[3] = lo[1] = lo[3] = 0;
-                    continue;
-                }
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float p0 = fast_exp2(s[n][2 * h] - base[h]), p1 = fast_exp2(s[n][2 * h + 1] - base[h]);
-                    l[h] += p0 + p1;
+                for (int h = 0; h < 2; ++h) {
+                    const float p0 = fast_exp2(s[b][2 * h] - base0), p1 = fast_exp2(s[b][2 * h + 1] - base1);
+                    l[b][0] += p0;
+                    l[b][1] += p1;
                     const uint32_t x = pack2<T>(p0, p1);
                     const float2 r = unpack2<T>(x);
-                    hi[2 * n + h] = x;
-                    lo[2 * n + h] = pack2<T>(p0 - r.x, p1 - r.y);
+                    hi[b][h] = transpose8x8(x);
+                    lo[b][h] = transpose8x8(pack2<T>(p0 - r.x, p1 - r.y));
                 }
             }
-            const uint32_t vaddr = vs + (lane & 15) * R::PITCH + (lane >> 4) * 16;
+            const uint32_t vaddr = vs + ((lane & 7) + (lane >> 4) * 8) * R::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                uint32_t b[4];
-                ldsm4_trans(b, vaddr + i * 32);
-                mma16816<T>(o[2 * i], hi, b[0], b[1]);
-                mma16816<T>(o[2 * i + 1], hi, b[2], b[3]);
-                mma16816<T>(o[2 * i], lo, b[0], b[1]);
-                mma16816<T>(o[2 * i + 1], lo, b[2], b[3]);
+                uint32_t v[4];
+                ldsm4_trans(v, vaddr + i * 32);
+#pragma unroll
+                for (int b = 0; b < NQ; ++b) {
+                    mma16816<T>(o[i][b], v, hi[b][0], hi[b][1]);
+                    mma16816<T>(o[i][b], v, lo[b][0], lo[b][1]);
+                }
             }
         }
         __syncwarp();
@@ -278,54 +299,74 @@ template <typename T, int D, int STAGES, int CTAS, bool WHOLE> __global__ void _
         // the piece ends here: hand this warp's part over, join the warps' parts, write
         fresh = true;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            const int r = qr + 8 * h;
-            if (r < rows) {
-                if ((lane & 3) == 0) {
-                    sm[warp][r] = m[h];
-                    sl[warp][r] = l[h];
-                }
-                float *p = so + (warp * a.merge_rows + r) * R::O_STRIDE + qc;
+        for (int b = 0; b < NQ; ++b)
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2 *>(p + i * 8) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+            for (int c = 0; c < 2; ++c) {
+                l[b][c] += __shfl_xor_sync(0xffffffffu, l[b][c], 4);
+                l[b][c] += __shfl_xor_sync(0xffffffffu, l[b][c], 8);
+                l[b][c] += __shfl_xor_sync(0xffffffffu, l[b][c], 16);
+                if (lr == 0) {
+                    sm[warp][b * 8 + lc + c] = m[b][c];
+                    sl[warp][b * 8 + lc + c] = l[b][c];
+                }
             }
-        }
         float *slot = nullptr;
         if (t0 > 0) {
-            slot = slot_of(a, blockIdx.x, 0, MMA_ROWS);
+            slot = slot_of(a, blockIdx.x, 0, ROWS);
         } else if (t1 < tiles) {
-            slot = slot_of(a, blockIdx.x, 1, MMA_ROWS);
+            slot = slot_of(a, blockIdx.x, 1, ROWS);
             if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), (int)((done - t1 + tiles - 1) / run.run), 0);
         }
-        __syncthreads();
-        write_piece<T, MMA_ROWS>(a, so, a.merge_rows * R::O_STRIDE, R::O_STRIDE, sm, sl, rows, seq, first_head, slot);
-        __syncthreads();
+        const int stride = part_stride(a.merge_dims);
+        for (int d0 = 0; d0 < D; d0 += a.merge_dims) {
+            float *part = so + warp * a.merge_rows * stride;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                if (i * 16 < d0 || i * 16 >= d0 + a.merge_dims) continue;
+#pragma unroll
+                for (int b = 0; b < NQ; ++b)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int r = b * 8 + lc + (x & 1);
+                        if (r < rows) part[r * stride + i * 16 - d0 + lr + (x >> 1) * 8] = o[i][b][x];
+                    }
+            }
+            __syncthreads();
+            write_piece<T, ROWS>(a, so, a.merge_rows * stride, stride, sm, sl, rows, seq, first_head, slot, d0, a.merge_dims);
+            __syncthreads();
+        }
     }
     cp_async_wait<0>();
     write_empty_rows<T>(a);
 }
 
-template <typename T, int D, int STAGES, int CTAS> int launch(PagedArgs a, int grid, cudaStream_t st) {
+// Shared memory of a CTA so that CTAS of them fit an SM (228 KB, 1 KB of it taken per CTA, and a little static).
+constexpr int budget(int ctas) { return (228 * 1024) / ctas - 1024 - 1280; }
+
+template <typename T, int D, int STAGES, int CTAS, int NQ> int launch(PagedArgs a, int grid, cudaStream_t st) {
     using R = Ring<D, STAGES>;
-    auto kern = a.whole ? paged_mma_kernel<T, D, STAGES, CTAS, true> : paged_mma_kernel<T, D, STAGES, CTAS, false>;
-    a.merge_rows = a.group < MMA_ROWS ? a.group : MMA_ROWS;
-    const int smem = R::TOTAL + WARPS * a.merge_rows * R::O_STRIDE * 4;
+    static_assert(R::TOTAL + WARPS * 8 * NQ * part_stride(D / 2) * 4 <= budget(CTAS), "partial results of half a head must fit");
+    auto kern = a.whole ? paged_mma_kernel<T, D, STAGES, CTAS, NQ, true> : paged_mma_kernel<T, D, STAGES, CTAS, NQ, false>;
+    a.merge_rows = a.group < 8 * NQ ? a.group : 8 * NQ;
+    a.merge_dims = R::TOTAL + WARPS * a.merge_rows * part_stride(D) * 4 <= budget(CTAS) ? D : D / 2;
+    const int smem = R::TOTAL + WARPS * a.merge_rows * part_stride(a.merge_dims) * 4;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail(ENC_ERR_LAUNCH, "enc_paged_attention: cannot opt in to %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
     launch_overlapped(kern, dim3(grid), dim3(THREADS), smem, st, a);
     return check_launch("enc_paged_attention");
 }
 
+template <typename T, int D, int STAGES1, int STAGES2, int CTAS> int launch_rows(const PagedArgs &a, int grid, cudaStream_t st) {
+    return mma_rows(a.group) == 8 ? launch<T, D, STAGES1, CTAS, 1>(a, grid, st) : launch<T, D, STAGES2, CTAS, 2>(a, grid, st);
+}
+
 template <typename T> int launch_dim(const PagedArgs &a, int grid, cudaStream_t st) {
     switch (a.head_dim) {
-        case 32: return launch<T, 32, 4, 2>(a, grid, st);
-        case 64: return launch<T, 64, 4, 2>(a, grid, st);
-        case 80: return launch<T, 80, 3, 2>(a, grid, st);
-        case 96: return launch<T, 96, 2, 2>(a, grid, st);
-        case 128: return launch<T, 128, 2, 2>(a, grid, st);
-        case 256: return launch<T, 256, 2, 1>(a, grid, st);
+        case 32: return launch_rows<T, 32, 4, 4, 3>(a, grid, st);
+        case 64: return launch_rows<T, 64, 3, 3, 3>(a, grid, st);
+        case 96: return launch_rows<T, 96, 3, 3, 2>(a, grid, st);
+        case 128: return launch_rows<T, 128, 3, 2, 2>(a, grid, st);
+        case 256: return launch_rows<T, 256, 2, 2, 1>(a, grid, st);
     }
     return fail(ENC_ERR_UNSUPPORTED, "enc_paged_attention: no tensor-core kernel for head_dim %d", a.head_dim);
 }
@@ -334,13 +375,16 @@ template <typename T> int launch_dim(const PagedArgs &a, int grid, cudaStream_t 
 
 int mma_ctas_per_sm(int64_t d) {
     switch (d) {
-        case 32: case 64: case 80: case 96: case 128: return 2;
+        case 32: case 64: return 3;
+        case 96: case 128: return 2;
         case 256: return 1;
     }
     return 0;
 }
 
-int launch_mma(const PagedArgs &a, int dtype, int grid, cudaStream_t st) {
+int launch_mma(const PagedArgs &args, int dtype, int grid, cudaStream_t st) {
+    PagedArgs a = args;
+    a.q_pairs = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && a.sq_s % 2 == 0 && a.sq_h % 2 == 0;
     return dtype == ENC_F16 ? launch_dim<__half>(a, grid, st) : launch_dim<__nv_bfloat16>(a, grid, st);
 }
 
