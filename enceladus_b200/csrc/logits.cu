@@ -4,10 +4,13 @@
 // penalty where positive and multiplied where not; one that was generated n > 0 times loses frequency * n + presence; the
 // row's biases are added; a token whose mask bit is clear becomes -inf whatever it was.
 //
-// What bounds it: bytes, the logits read once and written once.  A CTA owns a stretch of one row's vocabulary: it counts the
-// history's tokens that fall into the stretch in shared memory (integer atomics, so the order does not matter), then streams
-// the stretch; a count word of zero leaves the logit as it is, which is nearly all of them.  Nothing the size of the
-// vocabulary besides the logits touches memory.
+// What bounds it: bytes, the logits read once and written once.  A CTA owns a stretch of one row's vocabulary.  It streams the
+// stretch through the mask, which waits for nothing but the logits, and counts the history's tokens that fall into it in
+// shared memory meanwhile (integer atomics, so the order does not matter).  The tokens that something happens to are few but
+// scattered, and a warp that met them while streaming would walk through the penalties for one lane nearly every time (900
+// instructions a warp at 256 x 131072): so the thread that counts a token first puts it on a list, and the list is worked off
+// at the end with every lane busy, over what was streamed.  Nothing the size of the vocabulary besides the logits touches
+// memory.
 #include "paged.cuh"
 
 namespace enc {
@@ -26,6 +29,10 @@ struct LogitsArgs {
     int history, biases;
 };
 
+__device__ __forceinline__ float load_l2(const float *p) { return __ldcg(p); }
+__device__ __forceinline__ __half load_l2(const __half *p) { return __ldcg(p); }
+__device__ __forceinline__ __nv_bfloat16 load_l2(const __nv_bfloat16 *p) { return __ldcg(p); }
+
 // The logit of a token that its count word says something about.
 __device__ __forceinline__ float changed(float x, uint32_t w, float rep, float freq, float pres, const int32_t *ids, const float *values, int biases, int t) {
     const uint32_t n = w & COUNT;
@@ -43,15 +50,10 @@ __device__ __forceinline__ float changed(float x, uint32_t w, float rep, float f
 // VPT 16-byte vectors per thread: a stretch of VPT * THREADS vectors.  Stretches are cut so that the input's vectors are
 // aligned whatever the row's address: with `skew` elements of the row's first vector in front of the row, stretch i starts at
 // token i * TILE - skew.
-//
-// The tokens that something happens to are few but scattered: a warp streaming 32 vectors nearly always meets one, and the
-// whole warp would walk through the penalties for it, 900 instructions a warp at 256 x 131072.  So the thread that counts
-// a token first puts it on a list, the list is worked off with every lane busy, and the result goes back into the token's word
-// for the streaming loop to pick up.
 template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) logits_kernel(LogitsArgs a) {
     constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
-    extern __shared__ __align__(16) uint32_t seen[];  // [TILE] per token: what was counted, later ~(the bits of its new logit); 0: nothing
-    uint16_t *list = reinterpret_cast<uint16_t *>(seen + TILE);  // [TILE]
+    extern __shared__ __align__(16) uint32_t seen[];             // [TILE] what was counted per token
+    uint16_t *list = reinterpret_cast<uint16_t *>(seen + TILE);  // [TILE] the tokens with something counted
     __shared__ int listed;
     const int64_t row = blockIdx.y;
     const T *in = reinterpret_cast<const T *>(a.in) + row * a.s_in;
@@ -62,31 +64,27 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) log
     const int lo = v0 < 0 ? 0 : v0, hi = v0 + TILE < vocab ? v0 + TILE : vocab;  // tokens of the stretch
     const bool aligned_out = reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == skew;
     const int32_t *mask = a.mask ? a.mask + row * a.s_mask : nullptr;
+    const int32_t *tok = a.tokens + row * a.s_tokens;
+    const int history = a.tokens ? a.history : 0, h4 = aligned16(tok) ? history / 4 : 0;
     grid_dependency_wait();
     // Everything that the counting needs and the logits themselves are asked for at once: a stretch takes a few microseconds,
     // and one round trip to memory after the other would be most of them.
-    constexpr int UN = 4;  // vectors of the history in flight per thread
-    const int32_t *tok = a.tokens + row * a.s_tokens;
-    const int history = a.tokens ? a.history : 0, h4 = aligned16(tok) ? history / 4 : 0;
+    constexpr int UN = 2;  // vectors of the history in flight per thread
     const int4 nothing = make_int4(-1, -1, -1, -1);
     int4 token[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) token[u] = (int)threadIdx.x + u * THREADS < h4 ? reinterpret_cast<const int4 *>(tok)[threadIdx.x + u * THREADS] : nothing;
     int n = 0, prompt = 0;
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (a.tokens) {
         n = a.lens[row];
         prompt = a.prompt_lens[row];
-        rep = a.repetition[row];
-        freq = a.frequency[row];
-        pres = a.presence[row];
     }
     uint4 x[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int t = v0 + (j * THREADS + (int)threadIdx.x) * NV;
         if (t >= 0 && t + NV <= vocab) {
-            x[j] = *reinterpret_cast<const uint4 *>(in + t);
+            x[j] = ld_stream(in + t);
         } else {
             T *e = reinterpret_cast<T *>(&x[j]);
 #pragma unroll
@@ -101,7 +99,6 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) log
     bool bad = n < 0 || n > history || prompt < 0 || prompt > n;
     n = n < 0 ? 0 : n > history ? history : n;
     auto count = [&](int t, int i) {
-        if (i >= n) return;
         if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
             const uint32_t before = i < prompt ? atomicOr(&seen[t - v0], IN_PROMPT) : atomicAdd(&seen[t - v0], 1u);
             if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
@@ -117,11 +114,10 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) log
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const int at = 4 * (i + u * THREADS);
-            if (at >= n) break;
-            count(token[u].x, at);
-            count(token[u].y, at + 1);
-            count(token[u].z, at + 2);
-            count(token[u].w, at + 3);
+            if (at < n) count(token[u].x, at);
+            if (at + 1 < n) count(token[u].y, at + 1);
+            if (at + 2 < n) count(token[u].z, at + 2);
+            if (at + 3 < n) count(token[u].w, at + 3);
         }
     }
     for (int i = 4 * h4 + threadIdx.x; i < n; i += THREADS) count(tok[i], i);
@@ -136,43 +132,50 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) log
         }
     }
     if (bad && reports) atomicExch(&g_bad_index, 1u);
-    __syncthreads();
-    for (int i = threadIdx.x; i < listed; i += THREADS) {
-        const int at = list[i];
-        const float f = changed(to_f32(in[v0 + at]), seen[at], rep, freq, pres, ids, values, a.biases, v0 + at);
-        seen[at] = isnan(f) ? ~0x7fffffffu : ~__float_as_uint(f);  // (a NaN of all ones would read as nothing)
-    }
-    __syncthreads();
+
+    // the stream
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const int at = (j * THREADS + threadIdx.x) * NV, t = v0 + at;
+        const int t = v0 + (j * THREADS + (int)threadIdx.x) * NV;
         if (t + NV <= 0 || t >= vocab) continue;
-        uint32_t allowed = ~0u;
         if (mask) {  // NV bits from bit t on; bits in front of the row and behind it do not matter
-            const int first = t < 0 ? 0 : t, last = t + NV - 1 < vocab ? t + NV - 1 : vocab - 1;
-            const uint32_t lo = mask[first >> 5], hi = mask[last >> 5];
-            allowed = t < 0 ? lo << -t : __funnelshift_r(lo, hi, t & 31);
-        }
-        uint32_t words[NV];
-#pragma unroll
-        for (int i = 0; i < NV / 4; ++i) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(&seen[at + 4 * i]);
-            words[4 * i] = w.x; words[4 * i + 1] = w.y; words[4 * i + 2] = w.z; words[4 * i + 3] = w.w;
-        }
-        float f[NV];
-        Pack<T>::unpack(x[j], f);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (words[i]) f[i] = __uint_as_float(~words[i]);
-            if (!((allowed >> i) & 1)) f[i] = -INFINITY;
-        }
-        if (aligned_out && t >= 0 && t + NV <= vocab) {
-            *reinterpret_cast<uint4 *>(out + t) = Pack<T>::pack(f);
-        } else {
+            uint32_t allowed;
+            if (skew == 0) {
+                allowed = (uint32_t)mask[t >> 5] >> (t & 31);
+            } else {
+                const int first = t < 0 ? 0 : t, last = t + NV - 1 < vocab ? t + NV - 1 : vocab - 1;
+                const uint32_t w0 = mask[first >> 5], w1 = mask[last >> 5];
+                allowed = t < 0 ? w0 << -t : __funnelshift_r(w0, w1, t & 31);
+            }
+            float f[NV];
+            Pack<T>::unpack(x[j], f);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (t + i >= 0 && t + i < vocab) out[t + i] = from_f32<T>(f[i]);
+                if (!((allowed >> i) & 1)) f[i] = -INFINITY;
+            x[j] = Pack<T>::pack(f);
         }
+        if (aligned_out && t >= 0 && t + NV <= vocab) {
+            *reinterpret_cast<uint4 *>(out + t) = x[j];
+        } else {
+            const T *e = reinterpret_cast<const T *>(&x[j]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (t + i >= 0 && t + i < vocab) out[t + i] = e[i];
+        }
+    }
+    __syncthreads();
+    // the list; its logits come from L2 (in place, what was streamed over them is the same value, or -inf where -inf stays)
+    if (listed == 0) return;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (a.tokens) {
+        rep = a.repetition[row];
+        freq = a.frequency[row];
+        pres = a.presence[row];
+    }
+    for (int i = threadIdx.x; i < listed; i += THREADS) {
+        const int at = list[i], t = v0 + at;
+        const bool allowed = !mask || ((mask[t >> 5] >> (t & 31)) & 1);
+        if (allowed) out[t] = from_f32<T>(changed(to_f32(load_l2(in + t)), seen[at], rep, freq, pres, ids, values, a.biases, t));
     }
 }
 

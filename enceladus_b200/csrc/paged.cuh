@@ -2,7 +2,7 @@
 // records an index out of range, 16-byte asynchronous copies and the m16n8k16 matrix instruction.
 #pragma once
 
-#include "common.cuh"
+#include "sm100.cuh"
 
 namespace enc {
 
@@ -54,7 +54,7 @@ static inline int64_t paged_capacity(const enc_paged_cache &c) {
 }
 
 #ifdef __CUDACC__
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+using sm100::smem_u32;
 
 // 16 bytes global -> shared; with bytes == 0 nothing is read and 16 zero bytes are written.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {

@@ -9,61 +9,116 @@ using namespace paged;
 namespace {
 
 // ---- join ------------------------------------------------------------------------------------------
-// One CTA per (run, row): where a run's last piece begins a row group, the pieces of that group are that piece and the first
-// pieces of the runs after it.  Two passes over the pieces' statistics (maximum, then weights), then the weighted sum.
-template <typename T, int ROWS> __global__ void __launch_bounds__(THREADS) join_kernel(PagedArgs a) {
-    __shared__ float red[WARPS], part[WARPS][MAX_HEAD_DIM];
-    grid_dependency_wait();
-    const int4 h = a.headers[blockIdx.x];
-    const int rows = h.y & 255, first_head = h.y >> 8, r = blockIdx.y;
-    if (r >= rows) return;
-    const int n = h.z - (int)blockIdx.x + 1;  // pieces
+// Where a run's last piece begins a row group, the pieces of that group are that piece and the first pieces of the runs after
+// it.  A CTA looks through its share of the headers.  Rows cut into few pieces (up to JOIN_FEW) go to a warp each, all rows
+// of the CTA's headers side by side; rows cut into many (one long sequence has one per run) take the whole CTA, its warps
+// every JOIN_WARPS-th piece and then their results.  Lanes hold four neighbouring elements each; JOIN_DEEP pieces are in
+// flight per warp, because each is a trip to L2; one pass with a running maximum.
+constexpr int JOIN_WARPS = 8, JOIN_DEEP = 8, JOIN_FEW = 2 * JOIN_DEEP, JOIN_HEADERS = 64;
+
+struct Partial {
+    float x[4], m, l;
+};
+// Elements d .. d + 3 of the pieces first, first + step, ... of a row, joined.  pieces: piece 0 of the row's first run.
+__device__ __forceinline__ Partial join_pieces(const float *pieces, int64_t piece_stride, int ml_at, int d, int first, int n, int step) {
+    Partial s = {{0.0f, 0.0f, 0.0f, 0.0f}, -INFINITY, 0.0f};
+    for (int i = first; i < n; i += JOIN_DEEP * step) {
+        float4 y[JOIN_DEEP];
+        float2 ml[JOIN_DEEP];
+#pragma unroll
+        for (int u = 0; u < JOIN_DEEP; ++u) {
+            const int p = i + u * step;
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (p < n) {
+                const float *at = pieces + (p == 0 ? 1 : 2 * p) * piece_stride;
+                y[u] = *reinterpret_cast<const float4 *>(at + d);
+                ml[u] = *reinterpret_cast<const float2 *>(at + ml_at);
+            }
+        }
+        float top = s.m;
+#pragma unroll
+        for (int u = 0; u < JOIN_DEEP; ++u) top = fmaxf(top, ml[u].x);
+        const float base = top == -INFINITY ? 0.0f : top, down = fast_exp2(s.m - base);
+        s.m = top;
+        s.l *= down;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.x[e] *= down;
+#pragma unroll
+        for (int u = 0; u < JOIN_DEEP; ++u) {
+            const float w = fast_exp2(ml[u].x - base);
+            s.l = fmaf(ml[u].y, w, s.l);
+            s.x[0] = fmaf(y[u].x, w, s.x[0]); s.x[1] = fmaf(y[u].y, w, s.x[1]);
+            s.x[2] = fmaf(y[u].z, w, s.x[2]); s.x[3] = fmaf(y[u].w, w, s.x[3]);
+        }
+    }
+    return s;
+}
+template <typename T> __device__ __forceinline__ void write_row(const PagedArgs &a, int64_t seq, int head, int d, const Partial &s) {
+    store4<T>(reinterpret_cast<T *>(a.o) + seq * a.so_s + head * a.so_h, d, a.head_dim, s.x, s.l);
+    if (d == 0 && a.lse) a.lse[seq * a.q_heads + head] = s.l == 0.0f ? -INFINITY : (s.m + log2f(s.l)) * LN2;
+}
+
+template <typename T, int ROWS> __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(PagedArgs a, int grid) {
+    __shared__ int4 header[JOIN_HEADERS];
+    __shared__ Partial parts[JOIN_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t stride = a.head_dim + 2;
-    auto piece = [&](int i) { return slot_of(a, blockIdx.x + i, i == 0 ? 1 : 0, ROWS) + r * stride; };
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, piece(i)[a.head_dim]);
-    m = warp_max(m);
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
+    const int stride = (int)slot_stride(a.head_dim), width = stride - 4;  // floats of a row, elements
+    grid_dependency_wait();
+    for (int h0 = blockIdx.x; h0 < grid; h0 += JOIN_HEADERS * gridDim.x) {
+        const int left = (grid - h0 + (int)gridDim.x - 1) / (int)gridDim.x, count = left < JOIN_HEADERS ? left : JOIN_HEADERS;
+        __syncthreads();
+        if (threadIdx.x < count) {
+            const int id = h0 + threadIdx.x * gridDim.x, runs = a.headers[grid].x;
+            int4 h = a.headers[id];
+            if (id >= runs) h.y = 0;  // behind the last run with tiles nothing was written
+            h.w = h.z - id + 1;       // pieces
+            header[threadIdx.x] = h;
+        }
+        __syncthreads();
+        auto pieces_of = [&](int k, int r) { return slot_of(a, h0 + (int64_t)k * gridDim.x, 0, ROWS) + r * stride; };
+        for (int it = blockIdx.y * JOIN_WARPS + warp; it < count * ROWS; it += gridDim.y * JOIN_WARPS) {
+            const int k = it / ROWS, r = it % ROWS;
+            const int4 h = header[k];
+            if (r >= (h.y & 255) || h.w > JOIN_FEW) continue;
+            for (int d = lane * 4; d < width; d += 128)
+                write_row<T>(a, h.x, (h.y >> 8) + r, d, join_pieces(pieces_of(k, r), ROWS * stride, stride - 4, d, 0, h.w, 1));
+        }
+        for (int k = 0; k < count; ++k) {
+            const int4 h = header[k];
+            if ((h.y & 255) == 0 || h.w <= JOIN_FEW) continue;
+            for (int r = blockIdx.y; r < (h.y & 255); r += gridDim.y)
+                for (int d0 = 0; d0 < width; d0 += 128) {
+                    const int d = d0 + lane * 4;
+                    if (d < width) parts[warp][lane] = join_pieces(pieces_of(k, r), ROWS * stride, stride - 4, d, warp, h.w, JOIN_WARPS);
+                    __syncthreads();
+                    if (warp == 0 && d < width) {
+                        Partial s = parts[0][lane];
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, red[w]);
-    __syncthreads();
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, x[MAX_HEAD_DIM / 32];
+                        for (int w = 1; w < JOIN_WARPS; ++w) s.m = fmaxf(s.m, parts[w][lane].m);
+                        const float base = s.m == -INFINITY ? 0.0f : s.m;
+                        s.l = s.x[0] = s.x[1] = s.x[2] = s.x[3] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < MAX_HEAD_DIM / 32; ++i) x[i] = 0.0f;
-    for (int i = warp; i < n; i += WARPS) {  // a warp takes every WARPS-th piece, its lanes the elements
-        const float *p = piece(i);
-        const float c = fast_exp2(p[a.head_dim] - base);
-        l = fmaf(p[a.head_dim + 1], c, l);
+                        for (int w = 0; w < JOIN_WARPS; ++w) {
+                            const Partial &p = parts[w][lane];
+                            const float c = fast_exp2(p.m - base);
+                            s.l = fmaf(p.l, c, s.l);
 #pragma unroll
-        for (int j = 0; j < MAX_HEAD_DIM / 32; ++j)
-            if (lane + 32 * j < a.head_dim) x[j] = fmaf(p[lane + 32 * j], c, x[j]);
+                            for (int e = 0; e < 4; ++e) s.x[e] = fmaf(p.x[e], c, s.x[e]);
+                        }
+                        write_row<T>(a, h.x, (h.y >> 8) + r, d, s);
+                    }
+                    __syncthreads();
+                }
+        }
     }
-    if (lane == 0) red[warp] = l;
-#pragma unroll
-    for (int j = 0; j < MAX_HEAD_DIM / 32; ++j)
-        if (lane + 32 * j < a.head_dim) part[warp][lane + 32 * j] = x[j];
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) l += red[w];
-    const int64_t seq = h.x;
-    T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s + (first_head + r) * a.so_h;
-    for (int d = threadIdx.x; d < a.head_dim; d += THREADS) {
-        float y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) y += part[w][d];
-        o[d] = from_f32<T>(l == 0.0f ? 0.0f : __fdiv_rn(y, l));
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[seq * a.q_heads + first_head + r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
 // ---- CUDA-core kernel: any head_dim up to 256, any dtype, any strides ----------------------------------
 // Eight lanes share a key, four keys per warp at a time; a lane owns CH groups of four neighbouring elements of the head and
 // keeps its part of q and O for ROWS query rows in registers, with statistics of its own per group of eight lanes.  K and V
-// go straight from memory to registers.
+// go straight from memory to registers, KEYS keys per group at once: a step is a trip to memory, so what is in flight per
+// trip is what counts.
 template <typename T, bool VEC> __device__ __forceinline__ void load4(const T *p, int d, int head_dim, float (&f)[4]) {
     if (VEC) {
         if (sizeof(T) == 4) {
@@ -81,8 +136,12 @@ template <typename T, bool VEC> __device__ __forceinline__ void load4(const T *p
     }
 }
 
-template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bounds__(THREADS) paged_simple_kernel(PagedArgs a) {
-    __shared__ float so[WARPS * ROWS * MAX_HEAD_DIM], sm[WARPS][ROWS], sl[WARPS][ROWS];
+constexpr int cores_ctas_per_sm(int ch, int rows) { return ch * rows <= 2 ? 4 : ch * rows <= 8 ? 3 : 2; }
+
+template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bounds__(THREADS, cores_ctas_per_sm(CH, ROWS)) paged_simple_kernel(PagedArgs a) {
+    constexpr int KEYS = CH <= 2 ? 4 : CH == 4 ? 2 : 1;
+    __shared__ __align__(16) float so[WARPS * ROWS * MAX_HEAD_DIM];
+    __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, sub = lane >> 3;
     const int D = a.head_dim;
     grid_dependency_wait();
@@ -105,49 +164,74 @@ template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bound
                 }
             }
         }
+        // KEYS keys per group of lanes and step, all of their loads under way together; their pages are looked up a step ahead
         const int stop = t1 * TILE < keys ? t1 * TILE : keys;
-        for (int j0 = t0 * TILE + warp * 4; j0 < stop; j0 += 4 * WARPS) {  // the same trip count for the whole warp
-            const int j = j0 + sub;
-            int64_t page = 0;
-            int row = 0;
-            const bool in = j < stop && j >= skip && locate(a, seq, first + j, page, row);
-            float k[CH][4], v[CH][4];
+        int64_t place_page[KEYS];
+        int place_row[KEYS];
+        uint32_t there = 0;
+        auto look_up = [&](int j0) {
+            there = 0;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int d = (c * 8 + l8) * 4;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) k[c][e] = v[c][e] = 0.0f;
-                if (in && d < D) {
-                    load4<T, VEC>(kb + page * a.sk_p + row * a.sk_t, d, D, k[c]);
-                    load4<T, VEC>(vb + page * a.sv_p + row * a.sv_t, d, D, v[c]);
-                }
+            for (int u = 0; u < KEYS; ++u) {
+                const int j = j0 + 4 * u + sub;
+                place_page[u] = 0;
+                place_row[u] = 0;
+                if (j < stop && j >= skip && locate(a, seq, first + j, place_page[u], place_row[u])) there |= 1u << u;
             }
+        };
+        const int start = t0 * TILE + warp * 4 * KEYS;
+        look_up(start);
+        for (int j0 = start; j0 < stop; j0 += 4 * KEYS * WARPS) {  // the same trip count for the whole warp
+            float k[KEYS][CH][4], v[KEYS][CH][4];
+            const uint32_t in = there;
+#pragma unroll
+            for (int u = 0; u < KEYS; ++u)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int d = (c * 8 + l8) * 4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) k[u][c][e] = v[u][c][e] = 0.0f;
+                    if ((in >> u & 1) && d < D) {
+                        load4<T, VEC>(kb + place_page[u] * a.sk_p + place_row[u] * a.sk_t, d, D, k[u][c]);
+                        load4<T, VEC>(vb + place_page[u] * a.sv_p + place_row[u] * a.sv_t, d, D, v[u][c]);
+                    }
+                }
+            look_up(j0 + 4 * KEYS * WARPS);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
-                float s = 0.0f;
+                float s[KEYS], top = m[r];
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s = fmaf(q[r][c][e], k[c][e], s);
-                s += __shfl_xor_sync(0xffffffffu, s, 1);
-                s += __shfl_xor_sync(0xffffffffu, s, 2);
-                s += __shfl_xor_sync(0xffffffffu, s, 4);
-                if (!in) s = -INFINITY;
-                if (s > m[r]) {
-                    const float c0 = m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - s);
-                    m[r] = s;
-                    l[r] *= c0;
+                for (int u = 0; u < KEYS; ++u) {
+                    s[u] = 0.0f;
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[r][c][e] *= c0;
+                        for (int e = 0; e < 4; ++e) s[u] = fmaf(q[r][c][e], k[u][c][e], s[u]);
+                    s[u] += __shfl_xor_sync(0xffffffffu, s[u], 1);
+                    s[u] += __shfl_xor_sync(0xffffffffu, s[u], 2);
+                    s[u] += __shfl_xor_sync(0xffffffffu, s[u], 4);
+                    if (!(in >> u & 1)) s[u] = -INFINITY;
+                    top = fmaxf(top, s[u]);
                 }
-                const float p = in ? fast_exp2(s - (m[r] == -INFINITY ? 0.0f : m[r])) : 0.0f;
-                l[r] += p;
+                if (top > m[r]) {
+                    const float down = m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - top);
+                    m[r] = top;
+                    l[r] *= down;
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
+                    for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[r][c][e] = fmaf(p, v[c][e], o[r][c][e]);
+                        for (int e = 0; e < 4; ++e) o[r][c][e] *= down;
+                }
+                const float base = m[r] == -INFINITY ? 0.0f : m[r];
+#pragma unroll
+                for (int u = 0; u < KEYS; ++u) {
+                    const float p = fast_exp2(s[u] - base);
+                    l[r] += p;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[r][c][e] = fmaf(p, v[u][c][e], o[r][c][e]);
+                }
             }
         }
         // join the four groups of lanes, then hand the warp's result over
@@ -192,7 +276,7 @@ bool tensor_ok(const enc_paged_cache &c, int dtype) {
 }
 
 struct Plan {
-    int variant, rows, row_groups, grid;
+    int variant, rows, row_groups, long_runs, grid;
     int64_t work;
 };
 
@@ -201,18 +285,28 @@ void make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant
     const int group = (int)(q_heads / c.kv_heads);
     p.variant = variant >= 0 ? variant : tensor_ok(c, dtype) ? V_TENSOR : V_CORES;
     p.rows = p.variant == V_TENSOR ? mma_rows(group) : group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
-    const int per_sm = p.variant == V_TENSOR ? mma_ctas_per_sm(c.head_dim) : 4;
+    const int ch = c.head_dim > 128 ? 8 : c.head_dim > 64 ? 4 : 2;
+    const int per_sm = p.variant == V_TENSOR ? mma_ctas_per_sm(c.head_dim) : cores_ctas_per_sm(ch, p.rows);
     p.row_groups = (int)cdiv(group, p.rows);
     const int64_t most = c.num_seqs * c.kv_heads * p.row_groups * cdiv(paged_capacity(c), TILE);  // tiles if every row is full
     const int64_t fill = (int64_t)device_props().sm_count * per_sm;
-    p.grid = (int)(most < fill ? (most > 0 ? most : 1) : fill);
+    p.long_runs = (int)(most < fill ? (most > 0 ? most : 1) : fill);
+    // Short runs even out the SMs (see paged_attention.cuh) but cost two microseconds each: measured at 48 x 32 kv heads (664
+    // tiles a CTA at most) 685 us without, 637 with two per long run, 618 with six; at 64 x 8 (110 tiles) 105, 102, 140.  With
+    // fewer rows than CTAs every short run is a piece that the join has to fetch (2 x 4: 101 us without, 120 with two).
+    const int64_t units = c.num_seqs * c.kv_heads * p.row_groups;
+    const int shorts = p.variant != V_TENSOR || units < fill || most < 64 * fill ? 0 : most < 256 * fill ? 2 : 6;
+    p.grid = p.long_runs * (1 + shorts);
     // sequences of one tile are never cut
-    p.work = paged_capacity(c) <= TILE ? 0 : (int64_t)p.grid * 16 + 2 * (int64_t)p.grid * p.rows * (c.head_dim + 2) * 4;
+    p.work = paged_capacity(c) <= TILE ? 0 : (int64_t)(p.grid + 1) * 16 + 2 * (int64_t)p.grid * p.rows * slot_stride((int)c.head_dim) * 4;
 }
 
 template <typename T, int ROWS> void launch_join(const PagedArgs &a, int grid, cudaStream_t st) {
-    const int rows = a.group < ROWS ? a.group : ROWS;
-    if (a.headers) launch_overlapped(join_kernel<T, ROWS>, dim3(grid, rows), dim3(THREADS), 0, st, a);
+    if (!a.headers) return;
+    // CTAs side by side for the rows of a group where groups are cut into many pieces, so few of them have a header at all
+    const int most = 4 * device_props().sm_count;
+    const bool many = a.num_seqs * a.units * JOIN_FEW < grid;
+    launch_overlapped(join_kernel<T, ROWS>, dim3((unsigned)(grid < most ? grid : most), many ? (unsigned)(a.group < ROWS ? a.group : ROWS) : 1u), dim3(JOIN_WARPS * 32), 0, st, a, grid);
 }
 
 template <typename T, int CH, int ROWS>
@@ -259,6 +353,9 @@ int check_paged(const enc_paged_cache *c, int64_t q_heads, int dtype, int varian
     if (c->head_dim > MAX_HEAD_DIM) return fail(ENC_ERR_UNSUPPORTED, "%s: head_dim %lld > %d", me, (long long)c->head_dim, MAX_HEAD_DIM);
     if (q_heads < 1 || q_heads % c->kv_heads) return fail(ENC_ERR_BAD_ARG, "%s: %lld query heads over %lld kv heads", me, (long long)q_heads, (long long)c->kv_heads);
     if (q_heads > 0xffff) return fail(ENC_ERR_UNSUPPORTED, "%s: more than 65535 query heads", me);
+    if ((double)c->num_seqs * (double)q_heads * (double)cdiv(paged_capacity(*c), TILE) >= 2147400000.0)  // (room for a run more)
+        return fail(ENC_ERR_UNSUPPORTED, "%s: %lld sequences of up to %lld keys with %lld heads pass 2^31 tiles of %d keys", me,
+                    (long long)c->num_seqs, (long long)paged_capacity(*c), (long long)q_heads, TILE);
     if (variant == V_TENSOR && !tensor_ok(*c, dtype))
         return fail(ENC_ERR_UNSUPPORTED, "%s: variant %d needs float16 or bfloat16, another head_dim, or 16-byte aligned cache rows", me, variant);
     return 0;
@@ -306,7 +403,7 @@ extern "C" int enc_paged_attention(const enc_paged_cache *cache, const void *q, 
     a.q = q; a.k = cache->k; a.v = cache->v; a.o = o; a.lse = lse;
     a.block_table = cache->block_table; a.seq_lens = seq_lens;
     a.headers = p.work ? reinterpret_cast<int4 *>(work) : nullptr;
-    a.slots = p.work ? reinterpret_cast<float *>(reinterpret_cast<char *>(work) + (int64_t)p.grid * 16) : nullptr;
+    a.slots = p.work ? reinterpret_cast<float *>(reinterpret_cast<char *>(work) + (int64_t)(p.grid + 1) * 16) : nullptr;
     a.sq_s = q_stride_seq; a.sq_h = q_stride_head; a.so_s = o_stride_seq; a.so_h = o_stride_head;
     a.sk_p = cache->k_stride_page; a.sk_h = cache->k_stride_head; a.sk_t = cache->k_stride_token;
     a.sv_p = cache->v_stride_page; a.sv_h = cache->v_stride_head; a.sv_t = cache->v_stride_token;
@@ -315,7 +412,7 @@ extern "C" int enc_paged_attention(const enc_paged_cache *cache, const void *q, 
     a.q_heads = (int)q_heads; a.head_dim = (int)cache->head_dim; a.group = (int)(q_heads / cache->kv_heads);
     a.row_groups = p.row_groups; a.units = (int)cache->kv_heads * p.row_groups;
     a.whole = cache->page_size % 16 == 0;
-    a.min_run = 1;
+    a.long_runs = p.long_runs;
     a.scale = sm_scale * LOG2E;
     a.page_size = FastDiv((uint32_t)cache->page_size);
     cudaStream_t st = as_stream(stream);

@@ -8,12 +8,15 @@
 // What bounds it: each key and value is read once and used by the query heads that share it, a handful of operations per
 // byte, so the bound is HBM bandwidth; with few or short sequences, latency.
 //
-// Split: the work is a line of 64-key tiles (sequence by sequence, kv head by kv head), dealt out in equal contiguous
-// runs over a grid that fills the GPU once.  Every CTA finds its run from seq_lens by a scan over the batch, so ragged
-// lengths, one long sequence and many short ones all load every SM alike, and nothing about the lengths has to reach
-// the host.  A row that ends inside a run is finished there; the up to two pieces of a run that belong to rows cut by
-// its ends go to a workspace and a second, overlapped launch joins them in order (no atomics: the result does not depend
-// on timing).
+// Split: the work is a line of 64-key tiles (sequence by sequence, kv head by kv head), cut into runs.  Every CTA finds its
+// runs from seq_lens by a scan over the batch, so ragged lengths, one long sequence and many short ones all load every
+// SM alike, and nothing about the lengths has to reach the host.  A row that ends inside a run is finished there; the up to
+// two pieces of a run that belong to rows cut by its ends go to a workspace and a second, overlapped launch joins them in
+// order (no atomics: the result does not depend on timing).
+//
+// Equal runs are not equal times: SMs differ by up to 1.3 in the bandwidth they get (measured per SM with equal runs: 500 to
+// 663 us at 48 x 32 kv heads).  So the runs come in two lengths: as many long ones as CTAs fit the GPU, 60% of the work, and
+// several times as many short ones that the tensor-core kernel's CTAs claim as they get free (680 -> 617 us).
 #pragma once
 
 #include "paged.cuh"
@@ -31,14 +34,15 @@ struct PagedArgs {
     void *o;
     float *lse;
     const int32_t *block_table, *seq_lens;
-    int4 *headers;   // per CTA: the row group that its last piece begins {first query row, rows, last CTA of it, -}
-    float *slots;    // per CTA two pieces of `rows` x (head_dim + 2) floats: O, m, l
+    int4 *headers;   // per run: the row group that its last piece begins {sequence, rows and first head, last run of it, -};
+                     // behind the last run's, how many runs have tiles
+    float *slots;    // per run two pieces, see slot_of
     int64_t sq_s, sq_h, so_s, so_h, sk_p, sk_h, sk_t, sv_p, sv_h, sv_t, s_table;
     int64_t num_seqs, num_pages, capacity, window;
     int q_heads, head_dim, group, row_groups;  // query rows per kv head; row groups (of the kernel's row count) per kv head
     int units;                                 // row groups per sequence: kv_heads * row_groups
     bool whole;                                // pages are whole multiples of 16 keys
-    int min_run;                               // tiles a run has at least
+    int long_runs;                             // runs of the first kind; the grid's other runs are short ones
     bool q_pairs;                              // query elements can be read two at a time
     int merge_rows, merge_dims;                // rows and elements of a warp's part that shared memory holds at a time
     float scale;                               // sm_scale * log2(e)
@@ -60,104 +64,160 @@ static __device__ __forceinline__ int keys_of(const PagedArgs &a, int64_t b, int
     skip = begin - first;
     return n - first;
 }
-static __device__ __forceinline__ int64_t tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
+static __device__ __forceinline__ int tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
 
-struct Run {
-    int64_t seq, at;      // first sequence, first tile inside the sequence's units
-    int64_t begin, end;   // tiles on the line
-    int64_t run;          // tiles of a full run
+// The line of tiles, as every CTA computes it (below 2^31 tiles: the host refuses more, and 32-bit divisions are several times
+// as fast as 64-bit ones).
+struct Line {
+    int total, long_run, shorts_at, share;  // tiles; where the short runs begin and how many tiles they divide
+    int shorts;
+    bool any_empty;                         // some sequence has no keys
+
+    // A run's tiles; none if there are fewer tiles than runs, and then none in the runs behind it either.
+    __device__ __forceinline__ void run(const PagedArgs &a, int id, int &begin, int &end) const {
+        int64_t b, e;
+        if (id < a.long_runs) {
+            b = (int64_t)id * long_run;
+            e = b + long_run;
+        } else {  // the first `more` short runs have a tile more than the others
+            const int k = id - a.long_runs, least = share / shorts, more = share - least * shorts;
+            b = (int64_t)shorts_at + (int64_t)k * least + (k < more ? k : more);
+            e = b + least + (k < more);
+        }
+        begin = (int)(b < total ? b : total);
+        end = (int)(e < total ? e : total);
+    }
+    __device__ __forceinline__ int run_of(const PagedArgs &a, int tile) const {
+        if (tile < shorts_at) return tile / long_run;
+        const int least = share / shorts, more = share - least * shorts, x = tile - shorts_at, wide = more * (least + 1);
+        return a.long_runs + (x < wide ? x / (least + 1) : more + (x - wide) / least);
+    }
+    __device__ __forceinline__ int runs(const PagedArgs &a) const { return total > 0 ? run_of(a, total - 1) + 1 : 0; }
 };
 
-// Every thread of the CTA returns the CTA's run of tiles.  The sequences are dealt to the threads in contiguous pieces;
-// the thread whose piece holds the run's first tile finds the sequence.
-static __device__ __forceinline__ Run find_run(const PagedArgs &a) {
-    __shared__ int64_t warp_total[WARPS], found[2];
+// The sequences are dealt to the threads in contiguous pieces; `before`[i] (shared) becomes the tiles in front of thread i's
+// piece.
+static __device__ __forceinline__ Line make_line(const PagedArgs &a, int (&before)[THREADS]) {
+    __shared__ int warp_total[WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t per = (a.num_seqs + THREADS - 1) / THREADS;
     const int64_t b0 = threadIdx.x * per, b1 = b0 + per < a.num_seqs ? b0 + per : a.num_seqs;
-    int64_t mine = 0;
+    int mine = 0;
     int first, skip;
-    for (int64_t b = b0; b < b1; ++b) mine += tiles_of(keys_of(a, b, first, skip));
-    int64_t upto = mine;
+    bool empty = false;
+    for (int64_t b = b0; b < b1; ++b) {
+        const int keys = keys_of(a, b, first, skip);
+        empty |= keys == 0;
+        mine += tiles_of(keys) * a.units;
+    }
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
     }
     if (lane == 31) warp_total[warp] = upto;
-    __syncthreads();
-    int64_t total = 0, before = upto - mine;
+    Line r;
+    r.any_empty = __syncthreads_or(empty);
+    int front = upto - mine;
+    r.total = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) before += warp_total[w];
-        total += warp_total[w];
+        if (w < warp) front += warp_total[w];
+        r.total += warp_total[w];
     }
-    total *= a.units;
-    Run r;
-    r.run = (total + gridDim.x - 1) / gridDim.x;
-    if (r.run < a.min_run) r.run = a.min_run;
-    r.begin = blockIdx.x * r.run;
-    r.end = r.begin + r.run < total ? r.begin + r.run : total;
-    r.seq = r.at = 0;
-    if (r.begin >= r.end) return r;  // (the same for all threads: begin and end depend on the block alone)
-    if (before * a.units <= r.begin && r.begin < (before + mine) * a.units) {
-        int64_t at = r.begin - before * a.units;
-        for (int64_t b = b0; b < b1; ++b) {
-            const int64_t t = tiles_of(keys_of(a, b, first, skip)) * a.units;
-            if (at < t) {
-                found[0] = b;
-                found[1] = at;
-                break;
-            }
-            at -= t;
-        }
-    }
+    before[threadIdx.x] = front;
+    r.shorts = (int)gridDim.x - a.long_runs;
+    r.long_run = r.shorts > 0 ? r.total / 4 * 3 / a.long_runs : (r.total + a.long_runs - 1) / a.long_runs;
+    if (r.long_run < 1) r.long_run = 1;
+    r.shorts_at = r.long_run * a.long_runs;
+    r.share = r.total - r.shorts_at > r.shorts ? r.total - r.shorts_at : r.shorts;  // at least a tile each, to the last
+    if (threadIdx.x == 0 && a.headers) a.headers[gridDim.x].x = r.runs(a);  // for the join (the same from every block)
     __syncthreads();
-    r.seq = found[0];
-    r.at = found[1];
     return r;
 }
 
-static __device__ __forceinline__ float *slot_of(const PagedArgs &a, int64_t cta, int which, int rows) {
-    return a.slots + (2 * cta + which) * rows * (int64_t)(a.head_dim + 2);
+// The sequence that holds a tile of the line (tile < total), and the tile's place among the sequence's.  By a whole warp.
+static __device__ __forceinline__ void find_tile(const PagedArgs &a, const int (&before)[THREADS], int tile, int64_t &seq, int &at) {
+    const int lane = threadIdx.x & 31;
+    unsigned behind = 0;  // pieces that begin at the tile or in front of it
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) behind += before[lane + 32 * i] <= tile;
+    const int piece = (int)__reduce_add_sync(0xffffffffu, behind) - 1;
+    at = tile - before[piece];
+    seq = piece * ((a.num_seqs + THREADS - 1) / THREADS);
+    for (;; ++seq) {
+        int first, skip;
+        const int t = tiles_of(keys_of(a, seq, first, skip)) * a.units;
+        if (at < t) return;
+        at -= t;
+    }
 }
 
-// A piece's rows, one partial result per warp in shared memory (O unnormalised, rows `stride` apart, m and l),
-// joined and written (elements d0 .. d0 + dims - 1 of the head, `so` starting at d0): to the output when the piece is the whole row, to `slot` otherwise.
+// Elements e .. e + 3 of an output row of n: x / l, rounded once.
+template <typename T> __device__ __forceinline__ void store4(T *o, int e, int n, const float (&x)[4], float l) {
+    const float inverse = l == 0.0f ? 0.0f : __frcp_rn(l);
+    T y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(l == 0.0f ? 0.0f : x[i] * inverse);
+    if (e + 4 <= n && reinterpret_cast<uintptr_t>(o + e) % (4 * sizeof(T)) == 0) {
+        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(o + e) = reinterpret_cast<const uint4 &>(y);
+        else *reinterpret_cast<uint2 *>(o + e) = reinterpret_cast<const uint2 &>(y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (e + i < n) o[e + i] = y[i];
+    }
+}
+
+// A run's two pieces: `rows` rows of O (rounded up to four elements), then m and l.
+__host__ __device__ inline int64_t slot_stride(int head_dim) { return (head_dim + 3) / 4 * 4 + 4; }
+static __device__ __forceinline__ float *slot_of(const PagedArgs &a, int64_t run, int which, int rows) {
+    return a.slots + (2 * run + which) * rows * slot_stride(a.head_dim);
+}
+
+// A piece's rows, one partial result per warp in shared memory (O unnormalised, rows `stride` floats apart, m and l), joined and
+// written (elements d0 .. d0 + dims - 1 of the head, `so` starting at d0): to the output when the piece is the whole row, to
+// `slot` otherwise.  A warp per row, four neighbouring elements per lane; stride is a multiple of 4.
 template <typename T, int ROWS>
-static __device__ __forceinline__ void write_piece(const PagedArgs &a, const float *so, int warp_stride, int stride, const float (*sm)[ROWS], const float (*sl)[ROWS],
+__device__ __forceinline__ void write_piece(const PagedArgs &a, const float *so, int warp_stride, int stride, const float (*sm)[ROWS], const float (*sl)[ROWS],
                                             int rows, int64_t seq, int first_head, float *slot, int d0, int dims) {
-    T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s;
-    for (int i = threadIdx.x; i < rows * dims; i += THREADS) {
-        const int r = i / dims, e = i - r * dims, d = d0 + e;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r = warp; r < rows; r += WARPS) {
         float m = sm[0][r];
 #pragma unroll
         for (int w = 1; w < WARPS; ++w) m = fmaxf(m, sm[w][r]);
         const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, x = 0.0f;
+        float l = 0.0f, c[WARPS];
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float c = fast_exp2(sm[w][r] - base);
-            l = fmaf(sl[w][r], c, l);
-            x = fmaf(so[w * warp_stride + r * stride + e], c, x);
+            c[w] = fast_exp2(sm[w][r] - base);
+            l = fmaf(sl[w][r], c[w], l);
         }
-        if (slot) {
-            slot[r * (a.head_dim + 2) + d] = x;
-            if (d == 0) {
-                slot[r * (a.head_dim + 2) + a.head_dim] = m;
-                slot[r * (a.head_dim + 2) + a.head_dim + 1] = l;
+        T *o = reinterpret_cast<T *>(a.o) + seq * a.so_s + (first_head + r) * a.so_h + d0;
+        float *p = slot + r * slot_stride(a.head_dim);
+        for (int e = lane * 4; e < dims; e += 128) {
+            float x[4] = {};
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float4 y = *reinterpret_cast<const float4 *>(so + w * warp_stride + r * stride + e);
+                x[0] = fmaf(y.x, c[w], x[0]); x[1] = fmaf(y.y, c[w], x[1]);
+                x[2] = fmaf(y.z, c[w], x[2]); x[3] = fmaf(y.w, c[w], x[3]);
             }
-        } else {
-            o[(first_head + r) * a.so_h + d] = from_f32<T>(l == 0.0f ? 0.0f : __fdiv_rn(x, l));
-            if (d == 0 && a.lse) a.lse[seq * a.q_heads + first_head + r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+            if (slot) *reinterpret_cast<float4 *>(p + d0 + e) = make_float4(x[0], x[1], x[2], x[3]);
+            else store4<T>(o, e, dims, x, l);
+        }
+        if (lane == 0 && d0 == 0) {
+            if (slot) *reinterpret_cast<float2 *>(p + slot_stride(a.head_dim) - 4) = make_float2(m, l);
+            else if (a.lse) a.lse[seq * a.q_heads + first_head + r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
         }
     }
 }
 
-// The rows of sequences without keys, dealt over the grid: zero, lse -inf.
-template <typename T> __device__ __forceinline__ void write_empty_rows(const PagedArgs &a) {
+// The rows of sequences without keys, dealt over the long runs (which all have a block of their own): zero, lse -inf.
+template <typename T> __device__ __forceinline__ void write_empty_rows(const PagedArgs &a, int id) {
     T *o = reinterpret_cast<T *>(a.o);
-    for (int64_t b = blockIdx.x; b < a.num_seqs; b += gridDim.x) {  // rows without keys
+    for (int64_t b = id; b < a.num_seqs; b += a.long_runs) {
         int first, skip;
         if (keys_of(a, b, first, skip) > 0) continue;
         for (int i = threadIdx.x; i < a.q_heads * a.head_dim; i += THREADS) {
@@ -168,23 +228,25 @@ template <typename T> __device__ __forceinline__ void write_empty_rows(const Pag
     }
 }
 
-// Walks over the CTA's run: process(seq, kv head, first query head, rows, first key, keys to skip, keys, tile range, slot or NULL) per
-// piece.  Also writes the header that the join reads, and the rows of sequences without keys.
+// Walks over the CTA's run: process(seq, kv head, first query head, rows, first key, keys to skip, keys, tile range, slot or
+// NULL) per piece.  Also writes the header that the join reads, and the rows of sequences without keys.
 template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk_run(const PagedArgs &a, F process) {
-    const Run run = find_run(a);
+    __shared__ int before[THREADS];
+    const Line line = make_line(a, before);
+    int pos, end, at = 0;
+    int64_t seq = 0;
+    line.run(a, blockIdx.x, pos, end);
     if (threadIdx.x == 0 && a.headers) a.headers[blockIdx.x].y = 0;
-    int64_t seq = run.seq, at = run.at;
-    for (int64_t pos = run.begin; pos < run.end;) {
+    if (pos < end) find_tile(a, before, pos, seq, at);
+    while (pos < end) {
         int first, skip;
-        const int keys = keys_of(a, seq, first, skip);
-        const int64_t tiles = tiles_of(keys);
+        const int keys = keys_of(a, seq, first, skip), tiles = tiles_of(keys);
         if (at >= tiles * a.units) {
             at -= tiles * a.units;  // (zero: a sequence's tiles are walked to their end)
             ++seq;
             continue;
         }
-        const int unit = (int)(at / tiles), t0 = (int)(at - unit * tiles);
-        const int t1 = tiles - t0 < run.end - pos ? (int)tiles : t0 + (int)(run.end - pos);
+        const int unit = at / tiles, t0 = at - unit * tiles, t1 = tiles - t0 < end - pos ? tiles : t0 + (end - pos);
         const int kv_head = unit / a.row_groups, rg = unit - kv_head * a.row_groups;
         const int rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
         const int first_head = kv_head * a.group + rg * ROWS;
@@ -193,13 +255,13 @@ template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk
             slot = slot_of(a, blockIdx.x, 0, ROWS);
         } else if (t1 < tiles) {
             slot = slot_of(a, blockIdx.x, 1, ROWS);
-            if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), (int)((pos + tiles - 1) / run.run), 0);
+            if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), line.run_of(a, pos + tiles - 1), 0);
         }
         process(seq, kv_head, first_head, rows, first, skip, keys, t0, t1, slot);
         pos += t1 - t0;
         at += t1 - t0;
     }
-    write_empty_rows<T>(a);
+    if (line.any_empty) write_empty_rows<T>(a, blockIdx.x);
 }
 
 // Where key `pos` of sequence seq lives: its page and its row in it; false (and the error word) if the page is out of range.

@@ -54,20 +54,61 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x)
 }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(reinterpret_cast<const __half2 &>(x)); }
 
-// A place in the CTA's run: a tile of one unit (kv head and row group) of one sequence.
+// The runs of a CTA: its own block's first, then the runs of blocks that have not started, which it claims from the hardware's
+// queue (clusterlaunchcontrol: a claimed block never starts).  One claim is under way while a run is worked on; after a run
+// without tiles (there are none behind it) or a refusal no cursor claims more.  CLAIMS answers are kept: between the warps'
+// loading cursors lie at most STAGES tiles and two pieces, and a run has at least one tile.
+constexpr int CLAIMS = 16;
+struct Claims {
+    uint4 answer[CLAIMS];
+    uint64_t arrived[CLAIMS];
+    uint32_t gave_up;
+};
+__device__ __forceinline__ void claim(Claims &c, int i) {  // by one thread; i counts the CTA's runs
+    sm100::fence_proxy_async();
+    sm100::mbar_expect_tx(&c.arrived[i % CLAIMS], sizeof(uint4));
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(&c.answer[i % CLAIMS])), "r"(smem_u32(&c.arrived[i % CLAIMS])) : "memory");
+}
+// The i-th run's number, or -1 when there is none left (or the answer did not come within the bound of every wait).
+__device__ __forceinline__ int claimed(Claims &c, int i) {
+    if (!sm100::mbar_wait(&c.arrived[i % CLAIMS], (i / CLAIMS) & 1, &c.gave_up)) {
+        atomicExch(&g_bad_index, 2u);
+        return -1;
+    }
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t.reg .b128 A;\n\tld.shared.b128 A, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 P, A;\n\tselp.u32 %0, 1, 0, P;\n\tmov.u32 %1, 0;\n\t"
+        "@P clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, A;\n\t}"
+        : "=r"(ok), "=r"(x) : "r"(smem_u32(&c.answer[i % CLAIMS])) : "memory");
+    return ok ? (int)x : -1;
+}
+
+// A place in the CTA's runs: a tile of one unit (kv head and row group) of one sequence.
 struct Cursor {
-    int64_t left, seq;  // tiles left in the run
+    int64_t seq;
+    int left, end;           // tiles left in the run, the line's tile behind it
+    int run;                 // its number; -1: all done
     int unit, t, tiles, keys, first, skip;
 
-    __device__ __forceinline__ void start(const PagedArgs &a, const Run &run) {
-        left = run.end - run.begin;
-        if (left <= 0) return;
-        seq = run.seq;
+    __device__ __forceinline__ void read_keys(const PagedArgs &a) {
         keys = keys_of(a, seq, first, skip);
-        tiles = (int)tiles_of(keys);
-        unit = (int)(run.at / tiles);
-        t = (int)(run.at - (int64_t)unit * tiles);
+        tiles = tiles_of(keys);
     }
+    // Goes to run `id`, which may be empty.
+    __device__ __forceinline__ void start(const PagedArgs &a, const Line &line, const int (&before)[THREADS], int id) {
+        run = id;
+        int begin, at;
+        line.run(a, id, begin, end);
+        left = end - begin;
+        if (left <= 0) return;
+        find_tile(a, before, begin, seq, at);
+        read_keys(a);
+        unit = at / tiles;
+        t = at - unit * tiles;
+    }
+    // One tile on, inside the run.
     __device__ __forceinline__ void next(const PagedArgs &a) {
         --left;
         if (++t < tiles) return;
@@ -76,10 +117,13 @@ struct Cursor {
         unit = 0;
         do {  // (left > 0: a sequence with keys follows)
             ++seq;
-            keys = keys_of(a, seq, first, skip);
+            read_keys(a);
         } while (keys == 0);
-        tiles = (int)tiles_of(keys);
     }
+};
+// The runs that a warp's loading cursor has entered and its finishing cursor has not: at most one per stage, and one.
+template <int STAGES> struct RunQueue {
+    Cursor at[STAGES + 2];
 };
 
 template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global__ void __launch_bounds__(THREADS, CTAS) paged_mma_kernel(PagedArgs a) {
@@ -91,25 +135,73 @@ template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global_
     __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS];
     float *so = reinterpret_cast<float *>(smem + R::TOTAL);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t ring = smem_addr(smem) + warp * R::WARP;
+    const uint32_t ring = smem_u32(smem) + warp * R::WARP;
     const int lr = lane >> 2, lc = (lane & 3) * 2;  // this thread's row (and row + 8) and first column in accumulators
+    __shared__ Claims claims;
+    __shared__ RunQueue<STAGES> queue[WARPS];
+    __shared__ int before[THREADS];
+    const bool more = (int)gridDim.x > a.long_runs;  // there are runs to claim
+    if (threadIdx.x == 0 && more) {
+        for (int i = 0; i < CLAIMS; ++i) sm100::mbar_init(&claims.arrived[i], 1);
+        claims.gave_up = 0;
+        sm100::fence_barrier_init();
+    }
     grid_dependency_wait();
-    const Run run = find_run(a);
-    if (threadIdx.x == 0 && a.headers) a.headers[blockIdx.x].y = 0;
+    const Line line = make_line(a, before);  // (its barriers order the initialisation above, too)
+    if (threadIdx.x == 0 && more) claim(claims, 0);
 
-    Cursor load, at;
-    load.start(a, run);
-    at = load;
+    Cursor load, at;       // the tile that is loaded next, the tile that is worked on next
+    int entered = 0, finished = 0, answers = 0;  // runs that either has entered; claims looked at
+    bool queue_left = false;                     // the last run claimed had no tiles: others like it may wait
+    auto keep = [&]() {    // the loading cursor has entered a run (or come to the end)
+        if (lane == 0) queue[warp].at[entered % (STAGES + 2)] = load;
+        ++entered;
+        __syncwarp();
+    };
+    // Moves the loading cursor, at the end of its run, to the CTA's next.  The thread that learns of a run with tiles asks for
+    // the next.
+    auto next_run = [&]() {
+        const int id = more ? claimed(claims, answers) : -1;
+        ++answers;
+        load.run = -1;
+        if (id >= 0) {
+            load.start(a, line, before, id);
+            queue_left = load.left <= 0;
+            if (queue_left) {
+                if (line.any_empty && id < a.long_runs) write_empty_rows<T>(a, id);
+                load.run = -1;
+            } else if (threadIdx.x == 0) {
+                claim(claims, answers);
+            }
+        }
+        keep();
+    };
+    auto follow = [&]() {  // the finishing cursor enters the next run that the loading one has entered: what the run owes besides its tiles
+        at = queue[warp].at[finished % (STAGES + 2)];
+        ++finished;
+        if (at.run < 0) return;
+        if (threadIdx.x == 0 && a.headers) a.headers[at.run].y = 0;
+        if (line.any_empty && at.run < a.long_runs) write_empty_rows<T>(a, at.run);
+    };
+    load.start(a, line, before, blockIdx.x);
+    if (load.left > 0) {
+        keep();
+        follow();
+    } else {
+        if (line.any_empty && (int)blockIdx.x < a.long_runs) write_empty_rows<T>(a, blockIdx.x);
+        next_run();
+        follow();
+    }
     // Page number that the next copies need, read one tile ahead.  WHOLE: pages are whole multiples of 16 keys and so is the
     // first key, so a warp's 16 keys lie in one page and their rows at one distance; otherwise every lane looks up its key.
     int page = 0;
     auto read_page = [&]() {
-        if (load.left <= 0) return;
+        if (load.run < 0) return;
         const int j = load.t * TILE + warp * 16 + (WHOLE ? 0 : lane & 15);
         if (j < load.keys) page = a.block_table[load.seq * a.s_table + a.page_size.div((uint32_t)(load.first + j))];
     };
     auto issue = [&](int stage) {  // the copies of one tile's 16 keys and values, then one step on
-        if (load.left > 0) {
+        if (load.run >= 0) {
             const int j0 = load.t * TILE + warp * 16, n = load.keys - j0;  // keys of the 16 that exist
             const int kv_head = a.row_groups == 1 ? load.unit : load.unit / a.row_groups;
             const T *kb = reinterpret_cast<const T *>(a.k) + kv_head * a.sk_h, *vb = reinterpret_cast<const T *>(a.v) + kv_head * a.sv_h;
@@ -156,46 +248,67 @@ template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global_
                 }
             }
             load.next(a);
+            if (load.left <= 0) next_run();
             read_page();
         }
         cp_async_commit();
     };
-    read_page();
-#pragma unroll
-    for (int s = 0; s < STAGES; ++s) issue(s);
-
     uint32_t q[KS][NQ][2];
     float o[KS][NQ][4], m[NQ][2], l[NQ][2];  // O^T: rows i * 16 + lr (+ 8) of the head, columns lc, lc + 1 of the query block
-    bool fresh = true;
     int64_t seq = 0;
-    int first_head = 0, rows = 0, t0 = 0, stage = 0;
-    while (at.left > 0) {
-        if (fresh) {  // a new piece: its queries, and nothing seen yet
-            fresh = false;
-            seq = at.seq;
-            t0 = at.t;
-            const int kv_head = a.row_groups == 1 ? at.unit : at.unit / a.row_groups, rg = at.unit - kv_head * a.row_groups;
-            rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
-            first_head = kv_head * a.group + rg * ROWS;
-            const T *qp = reinterpret_cast<const T *>(a.q) + seq * a.sq_s + (int64_t)first_head * a.sq_h;
+    int first_head = 0, rows = 0, t0 = 0, stage = 0, discarded = 0;
+    auto begin_piece = [&]() {  // the finishing cursor stands at a piece's first tile: asks for its queries
+        seq = at.seq;
+        t0 = at.t;
+        const int kv_head = a.row_groups == 1 ? at.unit : at.unit / a.row_groups, rg = at.unit - kv_head * a.row_groups;
+        rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
+        first_head = kv_head * a.group + rg * ROWS;
+        const T *qp = reinterpret_cast<const T *>(a.q) + seq * a.sq_s + (int64_t)first_head * a.sq_h;
 #pragma unroll
-            for (int b = 0; b < NQ; ++b) {
-                const T *p = qp + (b * 8 + lr) * a.sq_h + lc;
-                const bool there = b * 8 + lr < rows;
+        for (int b = 0; b < NQ; ++b) {
+            const T *p = qp + (b * 8 + lr) * a.sq_h + lc;
+            const bool there = b * 8 + lr < rows;
 #pragma unroll
-                for (int i = 0; i < 2 * KS; ++i) {
-                    uint32_t v = 0;
-                    if (there && a.q_pairs) v = *reinterpret_cast<const uint32_t *>(p + i * 8);
-                    else if (there) v = (uint32_t)*reinterpret_cast<const uint16_t *>(p + i * 8) | (uint32_t)*reinterpret_cast<const uint16_t *>(p + i * 8 + 1) << 16;
-                    q[i / 2][b][i % 2] = v;
-                }
-                m[b][0] = m[b][1] = -INFINITY;
-                l[b][0] = l[b][1] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < KS; ++i)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) o[i][b][x] = 0.0f;
+            for (int i = 0; i < 2 * KS; ++i) {
+                uint32_t v = 0;
+                if (there && a.q_pairs) v = *reinterpret_cast<const uint32_t *>(p + i * 8);
+                else if (there) v = (uint32_t)*reinterpret_cast<const uint16_t *>(p + i * 8) | (uint32_t)*reinterpret_cast<const uint16_t *>(p + i * 8 + 1) << 16;
+                q[i / 2][b][i % 2] = v;
             }
+        }
+    };
+    auto clear = [&]() {  // nothing seen yet
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) {
+            m[b][0] = m[b][1] = -INFINITY;
+            l[b][0] = l[b][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[i][b][x] = 0.0f;
+        }
+    };
+    clear();
+    if (at.run >= 0) begin_piece();
+    for (bool prime = true;;) {
+        if (prime) {  // fill the ring
+            prime = false;
+            read_page();
+#pragma unroll 1
+            for (int s = 0; s < STAGES; ++s) issue(stage + s < STAGES ? stage + s : stage + s - STAGES);
+        }
+        if (at.run < 0) {
+            // Runs without tiles are at the queue's end and wait for nothing; taken off it, a bounded number by each CTA, they
+            // cost a claim instead of the start of a block.  All cursors stand here, so they go on together.
+            if (!queue_left || discarded++ == 32) break;
+            queue_left = false;
+            __syncthreads();
+            if (threadIdx.x == 0) claim(claims, answers);
+            next_run();
+            follow();
+            prime = at.run >= 0;
+            if (prime) begin_piece();
+            continue;
         }
         cp_async_wait<STAGES - 1>();
         __syncwarp();
@@ -292,12 +405,12 @@ template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global_
         issue(stage);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
 
-        const int t1 = at.t + 1, tiles = at.tiles;
-        const int64_t done = run.end - at.left + 1;  // tiles of the line up to here
+        const int t1 = at.t + 1, tiles = at.tiles, run = at.run;
+        const int done = at.end - at.left + 1;  // tiles of the line up to here
         at.next(a);
         if (t1 < tiles && at.left > 0) continue;
-        // the piece ends here: hand this warp's part over, join the warps' parts, write
-        fresh = true;
+        // the piece ends here: hand this warp's part over, join the warps' parts, write; the next piece's queries are under way
+        // meanwhile
 #pragma unroll
         for (int b = 0; b < NQ; ++b)
 #pragma unroll
@@ -312,12 +425,15 @@ template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global_
             }
         float *slot = nullptr;
         if (t0 > 0) {
-            slot = slot_of(a, blockIdx.x, 0, ROWS);
+            slot = slot_of(a, run, 0, ROWS);
         } else if (t1 < tiles) {
-            slot = slot_of(a, blockIdx.x, 1, ROWS);
-            if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), (int)((done - t1 + tiles - 1) / run.run), 0);
+            slot = slot_of(a, run, 1, ROWS);
+            if (threadIdx.x == 0) a.headers[run] = make_int4((int)seq, rows | (first_head << 8), line.run_of(a, done - t1 + tiles - 1), 0);
         }
-        const int stride = part_stride(a.merge_dims);
+        const int64_t old_seq = seq;
+        const int old_head = first_head, old_rows = rows, stride = part_stride(a.merge_dims);
+        if (at.left <= 0) follow();
+        if (at.run >= 0) begin_piece();
         for (int d0 = 0; d0 < D; d0 += a.merge_dims) {
             float *part = so + warp * a.merge_rows * stride;
 #pragma unroll
@@ -328,27 +444,27 @@ template <typename T, int D, int STAGES, int CTAS, int NQ, bool WHOLE> __global_
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const int r = b * 8 + lc + (x & 1);
-                        if (r < rows) part[r * stride + i * 16 - d0 + lr + (x >> 1) * 8] = o[i][b][x];
+                        if (r < old_rows) part[r * stride + i * 16 - d0 + lr + (x >> 1) * 8] = o[i][b][x];
                     }
             }
             __syncthreads();
-            write_piece<T, ROWS>(a, so, a.merge_rows * stride, stride, sm, sl, rows, seq, first_head, slot, d0, a.merge_dims);
+            write_piece<T, ROWS>(a, so, a.merge_rows * stride, stride, sm, sl, old_rows, old_seq, old_head, slot, d0, a.merge_dims);
             __syncthreads();
         }
+        clear();
     }
     cp_async_wait<0>();
-    write_empty_rows<T>(a);
 }
 
 // Shared memory of a CTA so that CTAS of them fit an SM (228 KB, 1 KB of it taken per CTA, and a little static).
-constexpr int budget(int ctas) { return (228 * 1024) / ctas - 1024 - 1280; }
+constexpr int budget(int ctas, int nq) { return (228 * 1024) / ctas - 1024 - (2304 + 256 * nq); }
 
 template <typename T, int D, int STAGES, int CTAS, int NQ> int launch(PagedArgs a, int grid, cudaStream_t st) {
     using R = Ring<D, STAGES>;
-    static_assert(R::TOTAL + WARPS * 8 * NQ * part_stride(D / 2) * 4 <= budget(CTAS), "partial results of half a head must fit");
+    static_assert(R::TOTAL + WARPS * 8 * NQ * part_stride(D / 2) * 4 <= budget(CTAS, NQ), "partial results of half a head must fit");
     auto kern = a.whole ? paged_mma_kernel<T, D, STAGES, CTAS, NQ, true> : paged_mma_kernel<T, D, STAGES, CTAS, NQ, false>;
     a.merge_rows = a.group < 8 * NQ ? a.group : 8 * NQ;
-    a.merge_dims = R::TOTAL + WARPS * a.merge_rows * part_stride(D) * 4 <= budget(CTAS) ? D : D / 2;
+    a.merge_dims = R::TOTAL + WARPS * a.merge_rows * part_stride(D) * 4 <= budget(CTAS, NQ) ? D : D / 2;
     const int smem = R::TOTAL + WARPS * a.merge_rows * part_stride(a.merge_dims) * 4;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail(ENC_ERR_LAUNCH, "enc_paged_attention: cannot opt in to %d bytes of shared memory: %s", smem, cudaGetErrorString(e));

@@ -253,6 +253,7 @@ extern "C" int enc_synchronize(void *stream) {
     }
     if (dev >= 0 && dev < enc::MAX_DEVICES && enc::g_indexed[dev].load(std::memory_order_relaxed)) {
         const unsigned append = enc::take_bad_index_append(), attend = enc::take_bad_index_paged_attention(), logits = enc::take_bad_index_logits();
+        if (attend & 2u) return enc::fail(ENC_ERR_DEVICE_WAIT, "enc_paged_attention: a device-side wait ran out of its iteration limit; results of the launches since the last synchronisation are invalid");
         if (append | attend | logits)
             return enc::fail(ENC_ERR_BAD_INDEX, "an index array held a value out of range (%s%s%s); what it named was skipped and results of the launches since the last synchronisation are incomplete",
                              append ? "enc_append_kv " : "", attend ? "enc_paged_attention " : "", logits ? "enc_penalize_logits " : "");

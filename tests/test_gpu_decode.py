@@ -306,6 +306,23 @@ def test_attention_many_sequences():
     check_attention(BF16, lens, heads=(4, 2), dim=64, page=16, variants=False, garbage=0.0)
 
 
+@pytest.mark.parametrize("columns", [200, 900])
+@pytest.mark.parametrize("longest", [0, 1, 40, 3000])
+def test_attention_wide_tables(columns, longest):
+    """Tables far wider than the lengths need: the grid is sized for rows that the lengths do not fill."""
+    r = np.random.default_rng(columns + longest)
+    lens = [int(x) for x in r.integers(0, longest + 1, 170)]
+    for dim, heads in ((64, (6, 3)), (128, (4, 4))):
+        check_attention(BF16, lens, heads=heads, dim=dim, page=16, variants=False, garbage=0.0, extra=columns, seed=longest)
+
+
+def test_attention_many_long_rows():
+    r = np.random.default_rng(1)
+    lens = [int(x) for x in r.integers(1, 6000, 100)]
+    check_attention(F16, lens, heads=(8, 8), dim=64, page=32, variants=False, garbage=0.0, extra=200, window=4000)
+    check_attention(BF16, lens, heads=(36, 4), dim=64, page=24, variants=False, garbage=0.0, extra=200)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
 def test_attention_growing_scores(dtype):
     """Scores spread over many powers of two, so that the running maximum moves and most weights are tiny."""
