@@ -4,21 +4,28 @@
 // penalty where positive and multiplied where not; one that was generated n > 0 times loses frequency * n + presence; the
 // row's biases are added; a token whose mask bit is clear becomes -inf whatever it was.
 //
-// What bounds it: bytes, the logits read once and written once.  A CTA owns a stretch of one row's vocabulary.  It streams the
-// stretch through the mask, which waits for nothing but the logits, and counts the history's tokens that fall into it in
-// shared memory meanwhile (integer atomics, so the order does not matter).  The tokens that something happens to are few but
-// scattered, and a warp that met them while streaming would walk through the penalties for one lane nearly every time (900
-// instructions a warp at 256 x 131072): so the thread that counts a token first puts it on a list, and the list is worked off
-// at the end with every lane busy, over what was streamed.  Nothing the size of the vocabulary besides the logits touches
-// memory.
+// What bounds it: bytes, the logits read once and written once.  Few tokens of a row are penalised, but they are scattered over
+// it, and whatever is done for one lane of a warp costs the warp.  So everything but the stream is done on compacted lists.
+// A CTA owns a stretch of one row's vocabulary.  It streams the stretch through the mask, which waits for nothing but the
+// logits.  Meanwhile it searches the row's history for tokens of the stretch (a comparison per token; a warp's finds take
+// their places in a queue by a prefix sum), counts the queue in shared memory (integer atomics, so the order does not
+// matter) and lists each token when it is first counted; the list is worked off over what was streamed and is still in L2.
+// Nothing the size of the vocabulary besides the logits touches memory.
+// Measured at 256 x 131072 float32 with histories up to 8192: penalties inside the stream 145 us, the list before the stream 131,
+// after it 102.  A second launch with a hash table per row 98 (its scattered reads and writes go to memory again), a cluster per
+// row that counts each token once over distributed shared memory 235 (common tokens queue up at one CTA).
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace enc {
 namespace {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr uint32_t IN_PROMPT = 1u << 31, HAS_BIAS = 1u << 30;          // above the count, which the history's length bounds
 constexpr uint32_t COUNT = HAS_BIAS - 1;
+constexpr int AHEAD = 8;                                               // tokens of the history per thread and round
+constexpr int STAGED = 512;                                            // biases that shared memory holds
 
 struct LogitsArgs {
     const void *in;
@@ -29,159 +36,243 @@ struct LogitsArgs {
     int history, biases;
 };
 
-__device__ __forceinline__ float load_l2(const float *p) { return __ldcg(p); }
-__device__ __forceinline__ __half load_l2(const __half *p) { return __ldcg(p); }
-__device__ __forceinline__ __nv_bfloat16 load_l2(const __nv_bfloat16 *p) { return __ldcg(p); }
-
-// The logit of a token that its count word says something about.
-__device__ __forceinline__ float changed(float x, uint32_t w, float rep, float freq, float pres, const int32_t *ids, const float *values, int biases, int t) {
-    const uint32_t n = w & COUNT;
-    if (n || (w & IN_PROMPT)) x = x > 0.0f ? __fdiv_rn(x, rep) : x * rep;
-    if (n) x -= fmaf(freq, (float)n, pres);
-    if (w & HAS_BIAS) {
-        float b = 0.0f;
-        for (int i = 0; i < biases; ++i)
-            if (ids[i] == t) b += values[i];
-        x += b;
+// A vector with -inf in place of the elements whose bits are clear.
+template <typename T> __device__ __forceinline__ uint4 masked(uint4 x, uint32_t bits) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = bits >> i & 1 ? w[i] : 0xff800000u;
+    } else {
+        const uint32_t low = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t keep = (bits >> (2 * i) & 1 ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
+            w[i] = (w[i] & keep) | (low & ~keep);
+        }
     }
     return x;
 }
 
-// VPT 16-byte vectors per thread: a stretch of VPT * THREADS vectors.  Stretches are cut so that the input's vectors are
-// aligned whatever the row's address: with `skew` elements of the row's first vector in front of the row, stretch i starts at
-// token i * TILE - skew.
+// A stretch of a row, cut so that the input's vectors are aligned whatever the row's address: with `skew` elements of the row's
+// first vector in front of the row, stretch i starts at token i * tile - skew.  A thread has VPT vectors of it.
+template <typename T, int VPT> struct Stretch {
+    static constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
+    const T *in;
+    T *out;
+    const int32_t *mask;
+    int skew, vocab, v0;  // v0: the stretch's first token; negative in a skewed row's first stretch
+    bool aligned_out;     // the input's vectors are vectors of the output too
+    bool inside;          // and all of them lie in the row
+    uint4 x[VPT];
+    uint32_t bits[VPT];   // the mask's
+
+    __device__ __forceinline__ Stretch(const LogitsArgs &a, int64_t row, int i) {
+        in = reinterpret_cast<const T *>(a.in) + row * a.s_in;
+        out = reinterpret_cast<T *>(a.out) + row * a.s_out;
+        mask = a.mask ? a.mask + row * a.s_mask : nullptr;
+        skew = (int)(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T));
+        vocab = (int)a.vocab;
+        v0 = i * TILE - skew;
+        aligned_out = reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == skew;
+        inside = v0 >= 0 && v0 + TILE <= vocab && aligned_out;
+    }
+    __device__ __forceinline__ int token(int j) const { return v0 + (j * THREADS + (int)threadIdx.x) * NV; }
+    __device__ __forceinline__ void load() {
+        if (inside) {
+            const T *p = in + v0 + (int)threadIdx.x * NV;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) x[j] = *reinterpret_cast<const uint4 *>(p + j * THREADS * NV);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int t = token(j);
+                if (t >= 0 && t + NV <= vocab) {
+                    x[j] = *reinterpret_cast<const uint4 *>(in + t);
+                } else {
+                    T *e = reinterpret_cast<T *>(&x[j]);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) e[i] = t + i >= 0 && t + i < vocab ? in[t + i] : from_f32<T>(0.0f);
+                }
+            }
+        }
+        if (!mask) return;
+        if (skew == 0) {  // a vector's bits lie in one word
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) bits[j] = token(j) < vocab ? (uint32_t)mask[token(j) >> 5] >> (token(j) & 31) : 0u;
+        } else {          // in two, perhaps; bits in front of the row and behind it do not matter
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int t = token(j), first = t < 0 ? 0 : t, last = t + NV - 1 < vocab ? t + NV - 1 : vocab - 1;
+                bits[j] = 0;
+                if (first > last) continue;
+                const uint32_t lo = mask[first >> 5], hi = mask[last >> 5];
+                bits[j] = t < 0 ? lo << -t : __funnelshift_r(lo, hi, t & 31);
+            }
+        }
+    }
+    __device__ __forceinline__ void store() {
+        if (mask) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) x[j] = masked<T>(x[j], bits[j]);
+        }
+        if (inside) {
+            T *p = out + v0 + (int)threadIdx.x * NV;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) *reinterpret_cast<uint4 *>(p + j * THREADS * NV) = x[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int t = token(j);
+                if (aligned_out && t >= 0 && t + NV <= vocab) {
+                    *reinterpret_cast<uint4 *>(out + t) = x[j];
+                } else {
+                    const T *e = reinterpret_cast<const T *>(&x[j]);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+                        if (t + i >= 0 && t + i < vocab) out[t + i] = e[i];
+                }
+            }
+        }
+    }
+};
+
+// VPT 16-byte vectors per thread: a stretch of VPT * THREADS vectors.
 template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) logits_kernel(LogitsArgs a) {
     constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
-    extern __shared__ __align__(16) uint32_t seen[];             // [TILE] what was counted per token
-    uint16_t *list = reinterpret_cast<uint16_t *>(seen + TILE);  // [TILE] the tokens with something counted
-    __shared__ int listed;
+    extern __shared__ __align__(16) uint32_t seen[];              // [TILE] what was counted per token
+    uint16_t *list = reinterpret_cast<uint16_t *>(seen + TILE);   // [TILE] the tokens with something counted
+    __shared__ uint16_t queue[THREADS * AHEAD];                   // finds of a round: place in the stretch, QUEUE_PROMPT
+    __shared__ int bias_id[STAGED], listed, queued;
+    __shared__ float bias_value[STAGED], penalty[3];
+    constexpr uint16_t QUEUE_PROMPT = 0x8000;
+    static_assert(TILE <= QUEUE_PROMPT, "a place and a flag in 16 bits");
+    const int lane = threadIdx.x & 31;
     const int64_t row = blockIdx.y;
-    const T *in = reinterpret_cast<const T *>(a.in) + row * a.s_in;
-    T *out = reinterpret_cast<T *>(a.out) + row * a.s_out;
-    const int skew = (int)(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T)), vocab = (int)a.vocab;
-    const int v0 = (int)blockIdx.x * TILE - skew;  // token of seen[0]; negative in a skewed row's first stretch
+    Stretch<T, VPT> st(a, row, blockIdx.x);
+    const int vocab = st.vocab, v0 = st.v0;
     if (v0 >= vocab) return;
     const int lo = v0 < 0 ? 0 : v0, hi = v0 + TILE < vocab ? v0 + TILE : vocab;  // tokens of the stretch
-    const bool aligned_out = reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == skew;
-    const int32_t *mask = a.mask ? a.mask + row * a.s_mask : nullptr;
-    const int32_t *tok = a.tokens + row * a.s_tokens;
-    const int history = a.tokens ? a.history : 0, h4 = aligned16(tok) ? history / 4 : 0;
+    const int32_t *tok = a.tokens + row * a.s_tokens, *ids = a.bias_ids + row * a.s_bias;
+    const float *values = a.bias_values + row * a.s_bias;
+    const int history = a.tokens ? a.history : 0;
+    const bool reports = blockIdx.x == 0;  // one CTA per row reports what is out of range
     grid_dependency_wait();
-    // Everything that the counting needs and the logits themselves are asked for at once: a stretch takes a few microseconds,
-    // and one round trip to memory after the other would be most of them.
-    constexpr int UN = 2;  // vectors of the history in flight per thread
-    const int4 nothing = make_int4(-1, -1, -1, -1);
-    int4 token[UN];
+    // Everything that the search needs and the logits themselves are asked for at once: a stretch takes a few microseconds, and
+    // one round trip to memory after the other would be most of them.
+    int token[AHEAD];
+    const bool quads = aligned16(tok) && history % 4 == 0;
+    auto load_tokens = [&](int i0) {  // AHEAD neighbouring tokens from i0 on, in fours
 #pragma unroll
-    for (int u = 0; u < UN; ++u) token[u] = (int)threadIdx.x + u * THREADS < h4 ? reinterpret_cast<const int4 *>(tok)[threadIdx.x + u * THREADS] : nothing;
+        for (int u = 0; u < AHEAD; u += 4) {
+            if (quads) {
+                int4 x = make_int4(0, 0, 0, 0);
+                if (i0 + u < history) x = *reinterpret_cast<const int4 *>(tok + i0 + u);
+                token[u] = x.x; token[u + 1] = x.y; token[u + 2] = x.z; token[u + 3] = x.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) token[u + e] = i0 + u + e < history ? tok[i0 + u + e] : 0;
+            }
+        }
+    };
+    load_tokens(threadIdx.x * AHEAD);
     int n = 0, prompt = 0;
     if (a.tokens) {
         n = a.lens[row];
         prompt = a.prompt_lens[row];
     }
-    uint4 x[VPT];
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int t = v0 + (j * THREADS + (int)threadIdx.x) * NV;
-        if (t >= 0 && t + NV <= vocab) {
-            x[j] = ld_stream(in + t);
-        } else {
-            T *e = reinterpret_cast<T *>(&x[j]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) e[i] = t + i >= 0 && t + i < vocab ? in[t + i] : from_f32<T>(0.0f);
-        }
+    for (int i = threadIdx.x; i < a.biases && i < STAGED; i += THREADS) {
+        bias_id[i] = ids[i];
+        bias_value[i] = values[i];
     }
+    if (threadIdx.x < 3 && a.tokens) penalty[threadIdx.x] = (threadIdx.x == 0 ? a.repetition : threadIdx.x == 1 ? a.frequency : a.presence)[row];
+    st.load();
 #pragma unroll
     for (int i = 0; i < TILE / 4 / THREADS; ++i) reinterpret_cast<uint4 *>(seen)[i * THREADS + threadIdx.x] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x == 0) listed = queued = 0;
     __syncthreads();
-    const bool reports = blockIdx.x == 0;  // one CTA per row reports what is out of range
     bool bad = n < 0 || n > history || prompt < 0 || prompt > n;
     n = n < 0 ? 0 : n > history ? history : n;
-    auto count = [&](int t, int i) {
-        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
-            const uint32_t before = i < prompt ? atomicOr(&seen[t - v0], IN_PROMPT) : atomicAdd(&seen[t - v0], 1u);
-            if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
-        } else if (reports) {
-            bad |= (unsigned)t >= (unsigned)vocab;
-        }
+    auto note = [&](int at, bool add, uint32_t what) {
+        const uint32_t before = add ? atomicAdd(&seen[at], what) : atomicOr(&seen[at], what);
+        if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)at;
     };
-    for (int i = threadIdx.x; i < h4 && 4 * i < n; i += UN * THREADS) {
-        if (i >= UN * THREADS) {
+    for (int r0 = 0; r0 < n; r0 += THREADS * AHEAD) {
+        const int i0 = r0 + threadIdx.x * AHEAD;
+        unsigned found = 0;
 #pragma unroll
-            for (int u = 0; u < UN; ++u) token[u] = i + u * THREADS < h4 ? reinterpret_cast<const int4 *>(tok)[i + u * THREADS] : nothing;
+        for (int u = 0; u < AHEAD; ++u)
+            if ((unsigned)(token[u] - lo) < (unsigned)(hi - lo)) found |= 1u << u;
+        const int here = n - i0;  // tokens of the AHEAD that count
+        const unsigned valid = here >= AHEAD ? (1u << AHEAD) - 1 : here > 0 ? (1u << here) - 1 : 0u;
+        found &= valid;
+        if (reports) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) bad |= (valid >> u & 1) && (unsigned)token[u] >= (unsigned)vocab;
         }
+        int before = __popc(found);  // inclusive prefix sum over the warp, one reservation per warp
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const int at = 4 * (i + u * THREADS);
-            if (at < n) count(token[u].x, at);
-            if (at + 1 < n) count(token[u].y, at + 1);
-            if (at + 2 < n) count(token[u].z, at + 2);
-            if (at + 3 < n) count(token[u].w, at + 3);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        int at = 0;
+        if (lane == 31 && before > 0) at = atomicAdd(&queued, before);
+        at = __shfl_sync(0xffffffffu, at, 31) + before - __popc(found);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (found >> u & 1) queue[at++] = (uint16_t)(token[u] - v0) | (i0 + u < prompt ? QUEUE_PROMPT : 0);
+        if (r0 + THREADS * AHEAD < n) load_tokens(i0 + THREADS * AHEAD);  // the next round's
+        __syncthreads();
+        const int in_queue = queued;
+        for (int i = threadIdx.x; i < in_queue; i += THREADS) {
+            const int q = queue[i];
+            note(q & (QUEUE_PROMPT - 1), !(q & QUEUE_PROMPT), q & QUEUE_PROMPT ? IN_PROMPT : 1u);
+        }
+        if (r0 + THREADS * AHEAD < n) {
+            __syncthreads();
+            if (threadIdx.x == 0) queued = 0;
+            __syncthreads();
         }
     }
-    for (int i = 4 * h4 + threadIdx.x; i < n; i += THREADS) count(tok[i], i);
-    const int32_t *ids = a.bias_ids + row * a.s_bias;
-    const float *values = a.bias_values + row * a.s_bias;
     for (int i = threadIdx.x; i < a.biases; i += THREADS) {
-        const int t = ids[i];
-        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) {
-            if (atomicOr(&seen[t - v0], HAS_BIAS) == 0) list[atomicAdd(&listed, 1)] = (uint16_t)(t - v0);
-        } else if (t < -1 || t >= vocab) {
-            bad = true;
-        }
+        const int t = i < STAGED ? bias_id[i] : ids[i];
+        if ((unsigned)(t - lo) < (unsigned)(hi - lo)) note(t - v0, false, HAS_BIAS);
+        else if (t < -1 || t >= vocab) bad = true;
     }
     if (bad && reports) atomicExch(&g_bad_index, 1u);
-
-    // the stream
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int t = v0 + (j * THREADS + (int)threadIdx.x) * NV;
-        if (t + NV <= 0 || t >= vocab) continue;
-        if (mask) {  // NV bits from bit t on; bits in front of the row and behind it do not matter
-            uint32_t allowed;
-            if (skew == 0) {
-                allowed = (uint32_t)mask[t >> 5] >> (t & 31);
-            } else {
-                const int first = t < 0 ? 0 : t, last = t + NV - 1 < vocab ? t + NV - 1 : vocab - 1;
-                const uint32_t w0 = mask[first >> 5], w1 = mask[last >> 5];
-                allowed = t < 0 ? w0 << -t : __funnelshift_r(w0, w1, t & 31);
-            }
-            float f[NV];
-            Pack<T>::unpack(x[j], f);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (!((allowed >> i) & 1)) f[i] = -INFINITY;
-            x[j] = Pack<T>::pack(f);
-        }
-        if (aligned_out && t >= 0 && t + NV <= vocab) {
-            *reinterpret_cast<uint4 *>(out + t) = x[j];
-        } else {
-            const T *e = reinterpret_cast<const T *>(&x[j]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (t + i >= 0 && t + i < vocab) out[t + i] = e[i];
-        }
-    }
+    st.store();
     __syncthreads();
-    // the list; its logits come from L2 (in place, what was streamed over them is the same value, or -inf where -inf stays)
+    // the list; its logits were read just now (in place, what was streamed over them is the same value, or -inf where -inf stays)
     if (listed == 0) return;
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if (a.tokens) {
-        rep = a.repetition[row];
-        freq = a.frequency[row];
-        pres = a.presence[row];
-    }
-    for (int i = threadIdx.x; i < listed; i += THREADS) {
-        const int at = list[i], t = v0 + at;
-        const bool allowed = !mask || ((mask[t >> 5] >> (t & 31)) & 1);
-        if (allowed) out[t] = from_f32<T>(changed(to_f32(load_l2(in + t)), seen[at], rep, freq, pres, ids, values, a.biases, t));
+    const float rep = penalty[0], freq = penalty[1], pres = penalty[2];  // (not looked at without a history)
+    for (int i0 = threadIdx.x - lane; i0 < listed; i0 += THREADS) {  // a warp's 32 of the list
+        const bool there = i0 + lane < listed;
+        const int at = there ? list[i0 + lane] : 0, t = v0 + at;
+        const uint32_t w = seen[at], made = w & COUNT;
+        const bool allowed = there && (!st.mask || ((st.mask[t >> 5] >> (t & 31)) & 1));
+        float f = allowed ? to_f32(st.in[t]) : 0.0f;
+        if (made || (w & IN_PROMPT)) f = f > 0.0f ? __fdiv_rn(f, rep) : f * rep;
+        if (made) f -= fmaf(freq, (float)made, pres);
+        // a token with biases: the warp searches them together and adds what it finds in their order
+        for (unsigned biased = __ballot_sync(0xffffffffu, allowed && (w & HAS_BIAS)); biased; biased &= biased - 1) {
+            const int who = __ffs(biased) - 1, wanted = __shfl_sync(0xffffffffu, t, who);
+            float b = 0.0f;
+            for (int e0 = 0; e0 < a.biases; e0 += 32) {
+                const int e = e0 + lane;
+                const int id = e >= a.biases ? -1 : e < STAGED ? bias_id[e] : ids[e];
+                for (unsigned hits = __ballot_sync(0xffffffffu, id == wanted); hits; hits &= hits - 1) {
+                    const int hit = e0 + __ffs(hits) - 1;
+                    b += hit < STAGED ? bias_value[hit] : values[hit];
+                }
+            }
+            if (lane == who) f += b;
+        }
+        if (allowed) st.out[t] = from_f32<T>(f);
     }
 }
 
 template <typename T, int VPT> void launch_tile(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
-    constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV;
-    constexpr int SMEM = TILE * 6;
+    constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV, SMEM = TILE * 6;
     cudaFuncSetAttribute(logits_kernel<T, VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     // a skewed row may need one stretch more
     launch_overlapped(logits_kernel<T, VPT>, dim3((unsigned)cdiv(a.vocab + NV - 1, TILE), (unsigned)rows), dim3(THREADS), SMEM, st, a);
@@ -199,7 +290,7 @@ template <typename T> int launch_logits(const LogitsArgs &a, int64_t rows, cudaS
 
 unsigned int take_bad_index_logits() { return take_bad_index_word(); }
 int logits_variants() { return 1; }
-void logits_variant_info(int, char *out, size_t n) { snprintf(out, n, "cta_threads=%d, counts of the history in shared memory", THREADS); }
+void logits_variant_info(int, char *out, size_t n) { snprintf(out, n, "cta_threads=%d, a stretch of the vocabulary per CTA", THREADS); }
 
 }  // namespace enc
 
