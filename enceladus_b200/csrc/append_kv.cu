@@ -197,53 +197,51 @@ void append_variant_info(int, char *out, size_t n) { snprintf(out, n, "one CTA o
 
 }  // namespace enc
 
-extern "C" int enc_append_kv(const enc_paged_cache *cache, const void *k, const void *v, const void *q, void *q_out,
-                             const float *cos, const float *sin, const int32_t *seq_ids, const int32_t *positions,
-                             int64_t tokens, int64_t q_heads, int64_t rot_dim, int interleaved, int64_t num_positions,
-                             int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
-                             int64_t q_stride_token, int64_t q_stride_head, int64_t o_stride_token, int64_t o_stride_head,
-                             int64_t stride_cos, int dtype, int variant, void *stream) {
+extern "C" int enc_append_kv(const enc_paged_cache *cache, const enc_append_args *args, int dtype, int variant, void *stream) {
     ENC_PROLOGUE();
     using namespace enc;
     const char *me = "enc_append_kv";
-    if (!cache) return fail(ENC_ERR_BAD_ARG, "%s: NULL cache", me);
+    if (!cache || !args) return fail(ENC_ERR_BAD_ARG, "%s: NULL cache or arguments", me);
+    const enc_append_args &g = *args;
+    const int64_t tokens = g.tokens, q_heads = g.q_heads, rot_dim = g.rot_dim;
+    const bool interleaved = g.interleaved != 0;
     if (!is_float_dtype(dtype)) return fail(ENC_ERR_BAD_ARG, "%s: dtype %d is not float16, bfloat16 or float32", me, dtype);
     if (variant >= append_variants()) return fail(ENC_ERR_BAD_ARG, "%s: variant %d out of range", me, variant);
     const int bad = check_cache(*cache, me);
     if (bad) return bad;
     if (tokens < 0 || q_heads < 0) return fail(ENC_ERR_BAD_ARG, "%s: negative size", me);
     if (rot_dim < 0 || rot_dim > cache->head_dim || rot_dim % 2) return fail(ENC_ERR_BAD_ARG, "%s: rot_dim %lld must be even and at most head_dim %lld", me, (long long)rot_dim, (long long)cache->head_dim);
-    if ((q != nullptr) != (q_out != nullptr)) return fail(ENC_ERR_BAD_ARG, "%s: q and q_out go together", me);
+    if ((g.q != nullptr) != (g.q_out != nullptr)) return fail(ENC_ERR_BAD_ARG, "%s: q and q_out go together", me);
     if (tokens == 0) return ENC_OK;
     if (tokens > 0x7fffffffLL || q_heads > 0xffff) return fail(ENC_ERR_UNSUPPORTED, "%s: more than 2^31-1 tokens or 65535 query heads", me);
-    if (!k || !v || !seq_ids || !positions) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
-    if (rot_dim > 0 && (!cos || !sin)) return fail(ENC_ERR_BAD_ARG, "%s: rot_dim %lld without cos and sin", me, (long long)rot_dim);
+    if (!g.k || !g.v || !g.seq_ids || !g.positions) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
+    if (rot_dim > 0 && (!g.cos || !g.sin)) return fail(ENC_ERR_BAD_ARG, "%s: rot_dim %lld without cos and sin", me, (long long)rot_dim);
     // (with no pages or no sequences nothing can be in range: the kernel reports every token that is not padding)
     if ((!cache->k || !cache->v || !cache->block_table) && cache->num_pages > 0 && cache->num_seqs > 0 && cache->table_width > 0)
         return fail(ENC_ERR_BAD_ARG, "%s: NULL cache tensor", me);
     AppendArgs a{};
-    a.k = k; a.v = v; a.q = q; a.q_out = q_out; a.k_cache = cache->k; a.v_cache = cache->v;
-    a.cos = cos; a.sin = sin; a.seq_ids = seq_ids; a.positions = positions; a.block_table = cache->block_table;
-    a.sk_t = k_stride_token; a.sk_h = k_stride_head; a.sv_t = v_stride_token; a.sv_h = v_stride_head;
-    a.sq_t = q_stride_token; a.sq_h = q_stride_head; a.so_t = o_stride_token; a.so_h = o_stride_head; a.s_cos = stride_cos;
+    a.k = g.k; a.v = g.v; a.q = g.q; a.q_out = g.q_out; a.k_cache = cache->k; a.v_cache = cache->v;
+    a.cos = g.cos; a.sin = g.sin; a.seq_ids = g.seq_ids; a.positions = g.positions; a.block_table = cache->block_table;
+    a.sk_t = g.k_stride_token; a.sk_h = g.k_stride_head; a.sv_t = g.v_stride_token; a.sv_h = g.v_stride_head;
+    a.sq_t = g.q_stride_token; a.sq_h = g.q_stride_head; a.so_t = g.o_stride_token; a.so_h = g.o_stride_head; a.s_cos = g.stride_cos;
     a.ck_p = cache->k_stride_page; a.ck_h = cache->k_stride_head; a.ck_t = cache->k_stride_token;
     a.cv_p = cache->v_stride_page; a.cv_h = cache->v_stride_head; a.cv_t = cache->v_stride_token;
     a.s_table = cache->stride_table;
-    a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.num_positions = num_positions;
+    a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.num_positions = g.num_positions;
     a.capacity = paged_capacity(*cache);
     a.q_heads = (int)q_heads; a.kv_heads = (int)cache->kv_heads; a.head_dim = (int)cache->head_dim; a.rot_dim = (int)rot_dim;
     a.page_size = FastDiv((uint32_t)cache->page_size);
-    a.angles_aligned = aligned16(cos) && aligned16(sin) && stride_cos % 4 == 0;
+    a.angles_aligned = aligned16(g.cos) && aligned16(g.sin) && g.stride_cos % 4 == 0;
     // 16-byte vectors where every row starts on 16 bytes and no vector straddles the rotated part or its halves
     const int nv = 16 / (int)dtype_size(dtype);
-    bool vec = cache->head_dim % nv == 0 && rot_dim % (interleaved ? nv : 2 * nv) == 0 && aligned16(k) && aligned16(v) &&
-               aligned16(cache->k) && aligned16(cache->v) && (!q || (aligned16(q) && aligned16(q_out)));
+    bool vec = cache->head_dim % nv == 0 && rot_dim % (interleaved ? nv : 2 * nv) == 0 && aligned16(g.k) && aligned16(g.v) &&
+               aligned16(cache->k) && aligned16(cache->v) && (!g.q || (aligned16(g.q) && aligned16(g.q_out)));
     for (int64_t s : {a.sk_t, a.sk_h, a.sv_t, a.sv_h, a.ck_p, a.ck_h, a.ck_t, a.cv_p, a.cv_h, a.cv_t}) vec = vec && s % nv == 0;
-    if (q) for (int64_t s : {a.sq_t, a.sq_h, a.so_t, a.so_h}) vec = vec && s % nv == 0;
+    if (g.q) for (int64_t s : {a.sq_t, a.sq_h, a.so_t, a.so_h}) vec = vec && s % nv == 0;
     cudaStream_t st = as_stream(stream);
     switch (dtype) {
-        case ENC_F16: return launch_append<__half>(a, tokens, interleaved != 0, vec, st);
-        case ENC_BF16: return launch_append<__nv_bfloat16>(a, tokens, interleaved != 0, vec, st);
-        default: return launch_append<float>(a, tokens, interleaved != 0, vec, st);
+        case ENC_F16: return launch_append<__half>(a, tokens, interleaved, vec, st);
+        case ENC_BF16: return launch_append<__nv_bfloat16>(a, tokens, interleaved, vec, st);
+        default: return launch_append<float>(a, tokens, interleaved, vec, st);
     }
 }

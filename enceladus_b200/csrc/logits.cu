@@ -294,30 +294,29 @@ void logits_variant_info(int, char *out, size_t n) { snprintf(out, n, "cta_threa
 
 }  // namespace enc
 
-extern "C" int enc_penalize_logits(const void *logits, void *out, int64_t rows, int64_t vocab, int64_t stride_in, int64_t stride_out,
-                                   const int32_t *tokens, int64_t history, int64_t stride_tokens, const int32_t *lens,
-                                   const int32_t *prompt_lens, const float *repetition, const float *frequency,
-                                   const float *presence, const int32_t *bias_ids, const float *bias_values, int64_t num_biases,
-                                   int64_t stride_bias, const int32_t *mask, int64_t stride_mask, int dtype, int variant, void *stream) {
+extern "C" int enc_penalize_logits(const enc_logits_args *args, int dtype, int variant, void *stream) {
     ENC_PROLOGUE();
     using namespace enc;
     const char *me = "enc_penalize_logits";
+    if (!args) return fail(ENC_ERR_BAD_ARG, "%s: NULL arguments", me);
+    const enc_logits_args &g = *args;
+    const int64_t rows = g.rows, vocab = g.vocab, history = g.history, num_biases = g.num_biases;
     if (!is_float_dtype(dtype)) return fail(ENC_ERR_BAD_ARG, "%s: dtype %d is not float16, bfloat16 or float32", me, dtype);
     if (variant >= logits_variants()) return fail(ENC_ERR_BAD_ARG, "%s: variant %d out of range", me, variant);
     if (rows < 0 || vocab < 0 || history < 0 || num_biases < 0) return fail(ENC_ERR_BAD_ARG, "%s: negative size", me);
-    const int given = !!tokens + !!lens + !!prompt_lens + !!repetition + !!frequency + !!presence;
-    if (given != 0 && given != 6 && !(given == 5 && !tokens && history == 0))
+    const int given = !!g.tokens + !!g.lens + !!g.prompt_lens + !!g.repetition + !!g.frequency + !!g.presence;
+    if (given != 0 && given != 6 && !(given == 5 && !g.tokens && history == 0))
         return fail(ENC_ERR_BAD_ARG, "%s: tokens, lens, prompt_lens, repetition, frequency and presence come together", me);
-    if (num_biases > 0 && (!bias_ids || !bias_values)) return fail(ENC_ERR_BAD_ARG, "%s: biases without ids or values", me);
-    if (mask && stride_mask < cdiv(vocab, 32)) return fail(ENC_ERR_BAD_ARG, "%s: %lld mask words a row do not cover %lld tokens", me, (long long)stride_mask, (long long)vocab);
+    if (num_biases > 0 && (!g.bias_ids || !g.bias_values)) return fail(ENC_ERR_BAD_ARG, "%s: biases without ids or values", me);
+    if (g.mask && g.stride_mask < cdiv(vocab, 32)) return fail(ENC_ERR_BAD_ARG, "%s: %lld mask words a row do not cover %lld tokens", me, (long long)g.stride_mask, (long long)vocab);
     if (rows == 0 || vocab == 0) return ENC_OK;
-    if (!logits || !out) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
+    if (!g.logits || !g.out) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
     if (rows > 65535 || vocab > 0x3fffffffLL || history > (int64_t)COUNT || num_biases > 0x3fffffffLL)
         return fail(ENC_ERR_UNSUPPORTED, "%s: more than 65535 rows, or 2^30-1 tokens, history or biases", me);
     LogitsArgs a{};
-    a.in = logits; a.out = out; a.tokens = tokens; a.lens = lens; a.prompt_lens = prompt_lens; a.bias_ids = bias_ids; a.mask = mask;
-    a.repetition = repetition; a.frequency = frequency; a.presence = presence; a.bias_values = bias_values;
-    a.vocab = vocab; a.s_in = stride_in; a.s_out = stride_out; a.s_tokens = stride_tokens; a.s_bias = stride_bias; a.s_mask = stride_mask;
+    a.in = g.logits; a.out = g.out; a.tokens = g.tokens; a.lens = g.lens; a.prompt_lens = g.prompt_lens; a.bias_ids = g.bias_ids; a.mask = g.mask;
+    a.repetition = g.repetition; a.frequency = g.frequency; a.presence = g.presence; a.bias_values = g.bias_values;
+    a.vocab = vocab; a.s_in = g.stride_in; a.s_out = g.stride_out; a.s_tokens = g.stride_tokens; a.s_bias = g.stride_bias; a.s_mask = g.stride_mask;
     a.history = (int)history; a.biases = (int)num_biases;
     cudaStream_t st = as_stream(stream);
     switch (dtype) {

@@ -375,45 +375,50 @@ void paged_attention_variant_info(int v, char *out, size_t n) {
 
 extern "C" int64_t enc_paged_attention_work_bytes(const enc_paged_cache *cache, int64_t q_heads, int dtype, int variant) {
     using namespace enc;
-    if (check_paged(cache, q_heads, dtype, variant, "enc_paged_attention_work_bytes")) return -1;
-    Plan p;
-    make_plan(*cache, q_heads, dtype, variant, p);
-    return p.work;
+    if (check_paged(cache, q_heads, dtype, variant < 0 ? -1 : V_CORES, "enc_paged_attention_work_bytes") || variant >= VARIANTS) return -1;
+    int64_t most = 0;
+    for (int v = 0; v < VARIANTS; ++v) {
+        if ((variant >= 0 && v != variant) || (v == V_TENSOR && (dtype_size(dtype) != 2 || mma_ctas_per_sm(cache->head_dim) == 0))) continue;
+        Plan p;
+        make_plan(*cache, q_heads, dtype, v, p);
+        if (p.work > most) most = p.work;
+    }
+    return most;
 }
 
-extern "C" int enc_paged_attention(const enc_paged_cache *cache, const void *q, void *o, float *lse, const int32_t *seq_lens,
-                                   int64_t q_heads, int64_t q_stride_seq, int64_t q_stride_head, int64_t o_stride_seq,
-                                   int64_t o_stride_head, float sm_scale, int64_t window, void *work, int64_t work_bytes,
-                                   int dtype, int variant, void *stream) {
+extern "C" int enc_paged_attention(const enc_paged_cache *cache, const enc_paged_attention_args *args, int dtype, int variant, void *stream) {
     ENC_PROLOGUE();
     using namespace enc;
     const char *me = "enc_paged_attention";
+    if (!args) return fail(ENC_ERR_BAD_ARG, "%s: NULL arguments", me);
+    const enc_paged_attention_args &g = *args;
+    const int64_t q_heads = g.q_heads;
     const int bad = check_paged(cache, q_heads, dtype, variant, me);
     if (bad) return bad;
-    if (window < 0) return fail(ENC_ERR_BAD_ARG, "%s: negative window", me);
+    if (g.window < 0) return fail(ENC_ERR_BAD_ARG, "%s: negative window", me);
     if (cache->num_seqs == 0) return ENC_OK;
-    if (!q || !o || !seq_lens) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
+    if (!g.q || !g.o || !g.seq_lens) return fail(ENC_ERR_BAD_ARG, "%s: NULL tensor", me);
     if ((!cache->k || !cache->v || !cache->block_table) && paged_capacity(*cache) > 0 && cache->num_pages > 0)
         return fail(ENC_ERR_BAD_ARG, "%s: NULL cache tensor", me);
     Plan p;
     make_plan(*cache, q_heads, dtype, variant, p);
-    if (p.work > 0 && (!work || work_bytes < p.work || !aligned16(work)))
-        return fail(ENC_ERR_BAD_ARG, "%s: needs %lld bytes of 16-byte aligned workspace, got %lld", me, (long long)p.work, (long long)work_bytes);
+    if (p.work > 0 && (!g.work || g.work_bytes < p.work || !aligned16(g.work)))
+        return fail(ENC_ERR_BAD_ARG, "%s: needs %lld bytes of 16-byte aligned workspace, got %lld", me, (long long)p.work, (long long)g.work_bytes);
     PagedArgs a{};
-    a.q = q; a.k = cache->k; a.v = cache->v; a.o = o; a.lse = lse;
-    a.block_table = cache->block_table; a.seq_lens = seq_lens;
-    a.headers = p.work ? reinterpret_cast<int4 *>(work) : nullptr;
-    a.slots = p.work ? reinterpret_cast<float *>(reinterpret_cast<char *>(work) + (int64_t)(p.grid + 1) * 16) : nullptr;
-    a.sq_s = q_stride_seq; a.sq_h = q_stride_head; a.so_s = o_stride_seq; a.so_h = o_stride_head;
+    a.q = g.q; a.k = cache->k; a.v = cache->v; a.o = g.o; a.lse = g.lse;
+    a.block_table = cache->block_table; a.seq_lens = g.seq_lens;
+    a.headers = p.work ? reinterpret_cast<int4 *>(g.work) : nullptr;
+    a.slots = p.work ? reinterpret_cast<float *>(reinterpret_cast<char *>(g.work) + (int64_t)(p.grid + 1) * 16) : nullptr;
+    a.sq_s = g.q_stride_seq; a.sq_h = g.q_stride_head; a.so_s = g.o_stride_seq; a.so_h = g.o_stride_head;
     a.sk_p = cache->k_stride_page; a.sk_h = cache->k_stride_head; a.sk_t = cache->k_stride_token;
     a.sv_p = cache->v_stride_page; a.sv_h = cache->v_stride_head; a.sv_t = cache->v_stride_token;
     a.s_table = cache->stride_table;
-    a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.capacity = paged_capacity(*cache); a.window = window;
+    a.num_seqs = cache->num_seqs; a.num_pages = cache->num_pages; a.capacity = paged_capacity(*cache); a.window = g.window;
     a.q_heads = (int)q_heads; a.head_dim = (int)cache->head_dim; a.group = (int)(q_heads / cache->kv_heads);
     a.row_groups = p.row_groups; a.units = (int)cache->kv_heads * p.row_groups;
     a.whole = cache->page_size % 16 == 0;
     a.long_runs = p.long_runs;
-    a.scale = sm_scale * LOG2E;
+    a.scale = (float)(g.sm_scale * 1.4426950408889634);
     a.page_size = FastDiv((uint32_t)cache->page_size);
     cudaStream_t st = as_stream(stream);
     switch (dtype) {

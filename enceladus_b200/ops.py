@@ -297,7 +297,7 @@ def _strides(x):
 
 def _straight(kernel, *arrays) -> int | None:
     """The stream for a straight call into the library, or None if the launch has to take the general path."""
-    if kernel.variant is not None or kernel.interpret is not None or os.environ.get("ENCELADUS_INTERPRET"):
+    if kernel.variant is not None or kernel.interpret is not None or "ENCELADUS_INTERPRET" in os.environ:
         return None
     return interop.direct_stream(*arrays)
 
@@ -403,7 +403,7 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_ids, positions, cos=None,
     stream = _straight(append_kv_kernel, k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin)
     if stream is not None:
         registry.append_kv(k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, tokens, seqs, width, st, pages,
-                           n_positions, k_st[:2], v_st[:2], q_st[:2], o_st[:2], cos_st, ks[:3], vs[:3], q_heads, kv_heads, d, rot_dim,
+                           n_positions, k_st, v_st, q_st, o_st, cos_st, ks, vs, q_heads, kv_heads, d, rot_dim,
                            page_size, 1 if interleaved else 0, -1, stream)
         return q_out
     append_kv_kernel[(tokens,)](k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, seqs, width, st, pages,
@@ -457,7 +457,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale: float 
     stream = _straight(paged_attention_kernel, q, k_cache, v_cache, o, lse, block_table, seq_lens)
     if stream is not None:
         registry.paged_attention(q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, seqs, block_table.shape[1], st, pages,
-                                 q_st[:2], o_st[:2], ks[:3], vs[:3], q_heads, kv_heads, d, page_size, -1, stream)
+                                 q_st, o_st, ks, vs, q_heads, kv_heads, d, page_size, -1, stream)
         return (o, lse) if return_lse else o
     paged_attention_kernel[(seqs,)](q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, block_table.shape[1], st, pages,
                                     q_st[0], q_st[1], o_st[0], o_st[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,

@@ -135,7 +135,7 @@ def _new_array(like: Any, shape: Any, dtype: Any, zero: bool) -> Any:
     if is_torch(like):
         torch = _torch()
         td = like.dtype if dtype is None else (dtype if isinstance(dtype, torch.dtype) else _np_to_torch_dtype(dtype))
-        return (torch.zeros if zero else torch.empty)(shape, dtype=td, device=like.device)
+        return (like.new_zeros if zero else like.new_empty)(shape, dtype=td)
     raise TypeError(_UNSUPPORTED.format(type(like).__name__))
 
 
@@ -203,12 +203,15 @@ def direct_stream(*arrays: Any) -> int | None:
     torch = _torch_mod
     if torch is None or not torch.cuda.is_initialized():
         return None
-    tensor = torch.Tensor
-    dev = torch._C._cuda_getDevice()
-    for a in arrays:
-        if a is not None and not (isinstance(a, tensor) and a.is_cuda and a.get_device() == dev):
-            return None
-    return current_stream()
+    dev = torch.cuda.current_device()
+    try:
+        for a in arrays:
+            if a is not None and a.get_device() != dev:  # (-1: in host memory)
+                return None
+    except AttributeError:  # a NumPy array, or no array at all
+        return None
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(dev) if raw is not None else current_stream()
 
 
 def _np_as_torch_view(a: np.ndarray):

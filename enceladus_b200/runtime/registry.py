@@ -11,6 +11,7 @@ point.  An unknown kernel raises `NotImplementedError`.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass, field
 from typing import Any, Callable
 
@@ -347,8 +348,8 @@ def _attention_lse(a, grid, variant, stream):
 # ---- the decoding step: paged cache, attention of one new token, logits -----------------------------
 # Each of the three calls below takes device tensors and sizes; the launch path reaches it through the adapter under it, the
 # wrapper in ops.py directly when there is nothing to stage.
-def _opt(t: Any) -> int | None:
-    return None if t is None else t.data_ptr()
+def _opt(t: Any) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _float_code(what: str, **arrays: Any) -> int:
@@ -378,13 +379,17 @@ def append_kv(k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions,
     i32 = torch.int32
     if not (block_table.dtype is i32 and seq_ids.dtype is i32 and positions.dtype is i32):
         _need(i32, block_table_ptr=block_table, seq_ids_ptr=seq_ids, positions_ptr=positions)
-    if cos is not None:
+    if cos is not None and not (cos.dtype is torch.float32 and sin.dtype is torch.float32):
         _need(torch.float32, cos_ptr=cos, sin_ptr=sin)
     cache = N.paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), n_pages, page_size, kv_heads, head_dim, n_seqs,
-                          table_width, stride_table, *kc_st, *vc_st)
-    N.check(N.load().enc_append_kv(cache, k.data_ptr(), v.data_ptr(), _opt(q), _opt(q_out), _opt(cos), _opt(sin), seq_ids.data_ptr(),
-                                   positions.data_ptr(), tokens, q_heads, rot_dim, interleaved, n_positions, *k_st, *v_st, *q_st, *o_st,
-                                   stride_cos, interop._TORCH_CODE[dt], variant, stream))
+                          table_width, stride_table, kc_st[0], kc_st[1], kc_st[2], vc_st[0], vc_st[1], vc_st[2])
+    args = N.append_args(k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr(),
+                         0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(),
+                         tokens, q_heads, rot_dim, interleaved, n_positions, k_st[0], k_st[1], v_st[0], v_st[1], q_st[0], q_st[1], o_st[0],
+                         o_st[1], stride_cos)
+    status = N.load().enc_append_kv(cache, args, interop._TORCH_CODE[dt], variant, stream)
+    if status:
+        N.check(status)
 
 
 def _ints(a: dict[str, Any], names: str) -> list[int]:
@@ -425,14 +430,22 @@ def paged_attention(q, k_cache, v_cache, o, lse, block_table, seq_lens, sm_scale
     if lse is not None:
         _need(torch.float32, lse_ptr=lse)
     cache = N.paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), n_pages, page_size, kv_heads, head_dim, seqs,
-                          table_width, stride_table, *kc_st, *vc_st)
-    code, lib = interop._TORCH_CODE[dt], N.load()
-    nbytes = lib.enc_paged_attention_work_bytes(cache, q_heads, code, variant)
-    work = None
-    if nbytes > 0:  # (a negative answer is a refusal, which the launch itself reports)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    N.check(lib.enc_paged_attention(cache, q.data_ptr(), o.data_ptr(), _opt(lse), seq_lens.data_ptr(), q_heads, *q_st, *o_st, sm_scale, window,
-                                    _opt(work), nbytes, code, variant, stream))
+                          table_width, stride_table, kc_st[0], kc_st[1], kc_st[2], vc_st[0], vc_st[1], vc_st[2])
+    code = interop._TORCH_CODE[dt]
+    nbytes = _work_bytes(q.get_device(), seqs, table_width, page_size, q_heads, kv_heads, head_dim, code, variant)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    args = N.paged_attention_args(q.data_ptr(), o.data_ptr(), _opt(lse), seq_lens.data_ptr(), _opt(work), nbytes, q_heads, q_st[0], q_st[1],
+                                  o_st[0], o_st[1], window, sm_scale)
+    status = N.load().enc_paged_attention(cache, args, code, variant, stream)
+    if status:
+        N.check(status)
+
+
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(device, seqs, table_width, page_size, q_heads, kv_heads, head_dim, code, variant) -> int:
+    """Workspace for a launch of these sizes on that (the current) device; 0 also where the launch itself will refuse them."""
+    cache = N.paged_cache(0, 0, 0, 0, page_size, kv_heads, head_dim, seqs, table_width, 0, 0, 0, 0, 0, 0, 0)
+    return max(0, N.load().enc_paged_attention_work_bytes(cache, q_heads, code, variant))
 
 
 # grid[0] = sequences
@@ -462,10 +475,12 @@ def penalize_logits(logits, out, tokens, lens, prompt_lens, repetition, frequenc
     for t in (repetition, frequency, presence, bias_values):
         if t is not None and t.dtype is not f32:
             _need(f32, repetition_ptr=repetition, frequency_ptr=frequency, presence_ptr=presence, bias_values_ptr=bias_values)
-    N.check(N.load().enc_penalize_logits(logits.data_ptr(), out.data_ptr(), rows, vocab, stride_in, stride_out, _opt(tokens), history,
-                                         stride_tokens, _opt(lens), _opt(prompt_lens), _opt(repetition), _opt(frequency), _opt(presence),
-                                         _opt(bias_ids), _opt(bias_values), n_biases, stride_bias, _opt(mask), stride_mask,
-                                         interop._TORCH_CODE[dt], variant, stream))
+    args = N.logits_args(logits.data_ptr(), out.data_ptr(), _opt(tokens), _opt(lens), _opt(prompt_lens), _opt(repetition), _opt(frequency),
+                         _opt(presence), _opt(bias_ids), _opt(bias_values), _opt(mask), rows, vocab, stride_in, stride_out, history,
+                         stride_tokens, n_biases, stride_bias, stride_mask)
+    status = N.load().enc_penalize_logits(args, interop._TORCH_CODE[dt], variant, stream)
+    if status:
+        N.check(status)
 
 
 # grid[0] = rows

@@ -245,7 +245,7 @@ typedef struct {
 
 /* Appends one key and one value per token to the cache and rotates queries and keys by their positions on the way.
  * Token t belongs to sequence seq_ids[t] and has position positions[t] in it; seq_ids[t] < 0 marks padding: nothing is
- * read or written for that token.  Of every query and key head the first rot_dim elements turn in pairs,
+ * written for that token.  Of every query and key head the first rot_dim elements turn in pairs,
  *   a' = a*cos - b*sin,  b' = b*cos + a*sin,   (a, b) = elements (i, i + rot_dim/2), or (2i, 2i+1) when `interleaved`,
  * in float32 with one rounding, by cos / sin [num_positions, rot_dim/2] (float32, rows stride_cos apart) at the token's
  * position; the other elements and the values are copied.  q and q_out may be NULL (no queries) or the same tensor;
@@ -255,18 +255,22 @@ typedef struct {
  * A token whose sequence, position or page is out of range is skipped and enc_synchronize returns ENC_ERR_BAD_INDEX.
  * Two tokens of one call must not name the same place in the cache: which of them stays there is not defined.
  * No counterpart in the reference, whose attention (examples/08_flash_attention.py:30-103) has no cache. */
-int enc_append_kv(const enc_paged_cache *cache, const void *k, const void *v, const void *q, void *q_out,
-                  const float *cos, const float *sin, const int32_t *seq_ids, const int32_t *positions,
-                  int64_t tokens, int64_t q_heads, int64_t rot_dim, int interleaved, int64_t num_positions,
-                  int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
-                  int64_t q_stride_token, int64_t q_stride_head, int64_t o_stride_token, int64_t o_stride_head,
-                  int64_t stride_cos, int dtype, int variant, void *stream);
+typedef struct {
+    const void *k, *v, *q;
+    void *q_out;
+    const float *cos, *sin;
+    const int32_t *seq_ids, *positions;
+    int64_t tokens, q_heads, rot_dim, interleaved, num_positions;
+    int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+    int64_t q_stride_token, q_stride_head, o_stride_token, o_stride_head, stride_cos;
+} enc_append_args;
+int enc_append_kv(const enc_paged_cache *cache, const enc_append_args *args, int dtype, int variant, void *stream);
 
 /* Attention of one new token per sequence over the cache: for every sequence s < cache->num_seqs and query head h,
  * o[s, h] = softmax(q[s, h] . K^T * sm_scale) V over the first seq_lens[s] tokens of the sequence (the last `window` of
  * them when window > 0), with head h reading kv head h / (q_heads / kv_heads).  Statistics and sums in float32.  A row
  * without keys (length zero), or whose weights sum to zero, is zero with lse -inf.  lse: float32 [num_seqs, q_heads] or
- * NULL.  Cache contents past a sequence's length are never used.
+ * NULL.  Cache contents past a sequence's length or in front of its window are never used.
  * q, o: [num_seqs, q_heads, head_dim] with strides per sequence and head; all of `dtype`; head_dim <= 256.
  * The keys of all sequences and heads are dealt out evenly over the GPU, whatever their lengths: the schedule is computed
  * on the device from seq_lens, so a captured launch follows the lengths it finds.  Pieces that do not finish a row go
@@ -274,11 +278,18 @@ int enc_append_kv(const enc_paged_cache *cache, const void *k, const void *v, co
  * no preparation and mean nothing afterwards; launches that may overlap need buffers of their own.
  * A length or page out of range is cut or skipped and enc_synchronize returns ENC_ERR_BAD_INDEX.
  * Counterpart in the reference for a whole sequence without a cache: examples/08_flash_attention.py:30-103 */
-int enc_paged_attention(const enc_paged_cache *cache, const void *q, void *o, float *lse, const int32_t *seq_lens,
-                        int64_t q_heads, int64_t q_stride_seq, int64_t q_stride_head, int64_t o_stride_seq,
-                        int64_t o_stride_head, float sm_scale, int64_t window, void *work, int64_t work_bytes,
-                        int dtype, int variant, void *stream);
-/* Bytes of `work` for enc_paged_attention with these arguments on the current device (0: none is needed); -1 on a bad argument. */
+typedef struct {
+    const void *q;
+    void *o;
+    float *lse;
+    const int32_t *seq_lens;
+    void *work;
+    int64_t work_bytes, q_heads, q_stride_seq, q_stride_head, o_stride_seq, o_stride_head, window;
+    double sm_scale;
+} enc_paged_attention_args;
+int enc_paged_attention(const enc_paged_cache *cache, const enc_paged_attention_args *args, int dtype, int variant, void *stream);
+/* Bytes of `work` that enc_paged_attention needs at most for caches and tables of these sizes (pointers and strides are not
+ * looked at) on the current device, 0: none; -1 on a bad argument. */
 int64_t enc_paged_attention_work_bytes(const enc_paged_cache *cache, int64_t q_heads, int dtype, int variant);
 
 /* Penalties, biases and grammar masks on logits [rows, vocab], one pass, float32 arithmetic, output in `dtype`:
@@ -292,11 +303,17 @@ int64_t enc_paged_attention_work_bytes(const enc_paged_cache *cache, int64_t q_h
  * mask [rows, stride_mask words] each may be NULL.  out may be logits itself.  Masked logits are -inf whatever they were.
  * A token, id or length out of range is ignored or cut and enc_synchronize returns ENC_ERR_BAD_INDEX.
  * No counterpart in the reference; the rows continue in softmax_kernel, examples/02_softmax.py:15-38 */
-int enc_penalize_logits(const void *logits, void *out, int64_t rows, int64_t vocab, int64_t stride_in, int64_t stride_out,
-                        const int32_t *tokens, int64_t history, int64_t stride_tokens, const int32_t *lens,
-                        const int32_t *prompt_lens, const float *repetition, const float *frequency,
-                        const float *presence, const int32_t *bias_ids, const float *bias_values, int64_t num_biases,
-                        int64_t stride_bias, const int32_t *mask, int64_t stride_mask, int dtype, int variant, void *stream);
+typedef struct {
+    const void *logits;
+    void *out;
+    const int32_t *tokens, *lens, *prompt_lens;
+    const float *repetition, *frequency, *presence;
+    const int32_t *bias_ids;
+    const float *bias_values;
+    const int32_t *mask;
+    int64_t rows, vocab, stride_in, stride_out, history, stride_tokens, num_biases, stride_bias, stride_mask;
+} enc_logits_args;
+int enc_penalize_logits(const enc_logits_args *args, int dtype, int variant, void *stream);
 
 /* ---- test hook ---------------------------------------------------------------------------- */
 

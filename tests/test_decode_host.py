@@ -28,31 +28,47 @@ def cache(**kw):
     return N.paged_cache(*(c[n] or 0 for n in N.PAGED_CACHE_FIELDS))
 
 
+def pack(what, fields, values):
+    return what(*(values[n] or 0 for n in fields))
+
+
 def append(lib, c, *, k=16, v=16, q=None, q_out=None, cos=None, sin=None, ids=16, pos=16, tokens=2, q_heads=0, rot=0, n_pos=0, dtype=N.F32,
            variant=-1):
-    return lib.enc_append_kv(c, k, v, q, q_out, cos, sin, ids, pos, tokens, q_heads, rot, 0, n_pos, 128, 64, 128, 64, 256, 64, 256, 64, 32,
-                             dtype, variant, None)
+    args = pack(N.append_args, N.APPEND_FIELDS, dict(
+        k=k, v=v, q=q, q_out=q_out, cos=cos, sin=sin, seq_ids=ids, positions=pos, tokens=tokens, q_heads=q_heads, rot_dim=rot, interleaved=0,
+        num_positions=n_pos, k_stride_token=128, k_stride_head=64, v_stride_token=128, v_stride_head=64, q_stride_token=256,
+        q_stride_head=64, o_stride_token=256, o_stride_head=64, stride_cos=32))
+    return lib.enc_append_kv(c, args, dtype, variant, None)
 
 
 def attend(lib, c, *, q=16, o=16, lens=16, q_heads=4, window=0, work=None, nbytes=0, dtype=N.F32, variant=-1):
-    return lib.enc_paged_attention(c, q, o, None, lens, q_heads, 256, 64, 256, 64, 0.125, window, work, nbytes, dtype, variant, None)
+    args = pack(N.paged_attention_args, N.PAGED_ATTENTION_FIELDS, dict(
+        q=q, o=o, lse=None, seq_lens=lens, work=work, work_bytes=nbytes, q_heads=q_heads, q_stride_seq=256, q_stride_head=64, o_stride_seq=256,
+        o_stride_head=64, window=window, sm_scale=0.125))
+    return lib.enc_paged_attention(c, args, dtype, variant, None)
 
 
 def logits(lib, *, x=16, out=16, rows=2, vocab=100, past=(None,) * 6, history=0, ids=None, values=None, biases=0, mask=None, words=4,
            dtype=N.F32, variant=-1):
-    return lib.enc_penalize_logits(x, out, rows, vocab, vocab, vocab, past[0], history, history, *past[1:], ids, values, biases, biases, mask,
-                                   words, dtype, variant, None)
+    args = pack(N.logits_args, N.LOGITS_FIELDS, dict(
+        logits=x, out=out, **dict(zip(("tokens", "lens", "prompt_lens", "repetition", "frequency", "presence"), past)), bias_ids=ids,
+        bias_values=values, mask=mask, rows=rows, vocab=vocab, stride_in=vocab, stride_out=vocab, history=history, stride_tokens=history,
+        num_biases=biases, stride_bias=biases, stride_mask=words))
+    return lib.enc_penalize_logits(args, dtype, variant, None)
 
 
-def test_struct_matches_the_header():
-    assert len(cache()) == 16 * 8 and ctypes.sizeof(ctypes.c_void_p) == 8
-    names = list(N.PAGED_CACHE_FIELDS)
-    text = (N.LIB_PATH.parents[2] / "include" / "enceladus_b200.h").read_text()
-    body = text[text.index("typedef struct {\n    void *k, *v;"):text.index("} enc_paged_cache;")]
+def test_structs_match_the_header():
     import re
 
-    body = re.sub(r"/\*.*?\*/", "", body)
-    assert [x for x in re.findall(r"\b\*?(\w+)\s*[,;]", body)] == names
+    text = (N.LIB_PATH.parents[2] / "include" / "enceladus_b200.h").read_text()
+    assert ctypes.sizeof(ctypes.c_void_p) == 8
+    for name, fields, size in (("enc_paged_cache", N.PAGED_CACHE_FIELDS, len(cache())), ("enc_append_args", N.APPEND_FIELDS, len(N.append_args(*[0] * 22))),
+                               ("enc_paged_attention_args", N.PAGED_ATTENTION_FIELDS, len(N.paged_attention_args(*[0] * 13))),
+                               ("enc_logits_args", N.LOGITS_FIELDS, len(N.logits_args(*[0] * 20)))):
+        end = text.index("} " + name + ";")
+        body = re.sub(r"/\*.*?\*/", "", text[text.rindex("typedef struct {", 0, end):end], flags=re.S)
+        assert re.findall(r"\b\*?(\w+)\s*[,;]", body) == list(fields), name
+        assert size == 8 * len(fields), name  # pointers, 64-bit integers and a double: no padding
     assert N.ERR_BAD_INDEX == 6 and "ENC_ERR_BAD_INDEX = 6" in text
     for name in ("APPEND_KV", "PAGED_ATTENTION", "LOGITS"):
         assert f"ENC_K_{name} = {getattr(N, 'K_' + name)}" in text
