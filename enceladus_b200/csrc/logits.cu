@@ -271,19 +271,20 @@ template <typename T, int VPT> __global__ void __launch_bounds__(THREADS, 3) log
     }
 }
 
-template <typename T, int VPT> void launch_tile(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
+template <typename T, int VPT> int launch_tile(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
     constexpr int NV = Pack<T>::N, TILE = VPT * THREADS * NV, SMEM = TILE * 6;
-    cudaFuncSetAttribute(logits_kernel<T, VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    static OncePerDevice opted;
+    const int rc = opted.opt_in(logits_kernel<T, VPT>, SMEM, "enc_penalize_logits");
+    if (rc != ENC_OK) return rc;
     // a skewed row may need one stretch more
     launch_overlapped(logits_kernel<T, VPT>, dim3((unsigned)cdiv(a.vocab + NV - 1, TILE), (unsigned)rows), dim3(THREADS), SMEM, st, a);
+    return check_launch("enc_penalize_logits");
 }
 
 template <typename T> int launch_logits(const LogitsArgs &a, int64_t rows, cudaStream_t st) {
     note_indexed_launch();
     constexpr int VPT = 8192 / THREADS / Pack<T>::N;
-    if (rows * cdiv(a.vocab, 8192) >= device_props().sm_count) launch_tile<T, VPT>(a, rows, st);
-    else launch_tile<T, 1>(a, rows, st);
-    return check_launch("enc_penalize_logits");
+    return rows * cdiv(a.vocab, 8192) >= device_props().sm_count ? launch_tile<T, VPT>(a, rows, st) : launch_tile<T, 1>(a, rows, st);
 }
 
 }  // namespace

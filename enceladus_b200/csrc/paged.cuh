@@ -2,6 +2,8 @@
 // records an index out of range, 16-byte asynchronous copies and the m16n8k16 matrix instruction.
 #pragma once
 
+#include <atomic>
+
 #include "sm100.cuh"
 
 namespace enc {
@@ -52,6 +54,22 @@ static inline int64_t paged_capacity(const enc_paged_cache &c) {
     const int64_t n = c.table_width * c.page_size;  // both below 2^31
     return n < 0x7fffff00LL ? n : 0x7fffff00LL;  // (room for the last tile in 32 bits)
 }
+
+// Opting in to more than 48 KB of shared memory, once per kernel and device instead of at every launch.
+struct OncePerDevice {
+    std::atomic<uint64_t> done{0};
+    template <typename K> int opt_in(K kernel, int bytes, const char *me) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const uint64_t bit = 1ull << (dev & 63);
+        if (done.load(std::memory_order_acquire) & bit) return ENC_OK;
+        const int most = device_props().max_smem_optin;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most > 0 && bytes > most ? most : bytes);
+        if (e != cudaSuccess) return fail(ENC_ERR_LAUNCH, "%s: cannot opt in to %d bytes of shared memory: %s", me, bytes, cudaGetErrorString(e));
+        done.fetch_or(bit, std::memory_order_release);
+        return ENC_OK;
+    }
+};
 
 #ifdef __CUDACC__
 using sm100::smem_u32;

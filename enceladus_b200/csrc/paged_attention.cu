@@ -278,6 +278,7 @@ bool tensor_ok(const enc_paged_cache &c, int dtype) {
 struct Plan {
     int variant, rows, row_groups, long_runs, grid;
     int64_t work;
+    bool by_rows;
 };
 
 // Which kernel, how many query rows it takes at a time, how many CTAs, and the bytes for pieces.
@@ -288,17 +289,17 @@ void make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant
     const int ch = c.head_dim > 128 ? 8 : c.head_dim > 64 ? 4 : 2;
     const int per_sm = p.variant == V_TENSOR ? mma_ctas_per_sm(c.head_dim) : cores_ctas_per_sm(ch, p.rows);
     p.row_groups = (int)cdiv(group, p.rows);
-    const int64_t most = c.num_seqs * c.kv_heads * p.row_groups * cdiv(paged_capacity(c), TILE);  // tiles if every row is full
+    const int64_t units = c.num_seqs * c.kv_heads * p.row_groups, row_tiles = cdiv(paged_capacity(c), TILE);
+    p.by_rows = row_tiles <= ROW_TILES;
+    const int64_t most = p.by_rows ? units : units * row_tiles;  // the line's length if every row is full
     const int64_t fill = (int64_t)device_props().sm_count * per_sm;
     p.long_runs = (int)(most < fill ? (most > 0 ? most : 1) : fill);
     // Short runs even out the SMs (see paged_attention.cuh) but cost two microseconds each: measured at 48 x 32 kv heads (664
     // tiles a CTA at most) 685 us without, 637 with two per long run, 618 with six; at 64 x 8 (110 tiles) 105, 102, 140.  With
     // fewer rows than CTAs every short run is a piece that the join has to fetch (2 x 4: 101 us without, 120 with two).
-    const int64_t units = c.num_seqs * c.kv_heads * p.row_groups;
-    const int shorts = p.variant != V_TENSOR || units < fill || most < 64 * fill ? 0 : most < 256 * fill ? 2 : 6;
+    const int shorts = p.variant != V_TENSOR || p.by_rows || units < fill || most < 64 * fill ? 0 : most < 256 * fill ? 2 : 6;
     p.grid = p.long_runs * (1 + shorts);
-    // sequences of one tile are never cut
-    p.work = paged_capacity(c) <= TILE ? 0 : (int64_t)(p.grid + 1) * 16 + 2 * (int64_t)p.grid * p.rows * slot_stride((int)c.head_dim) * 4;
+    p.work = p.by_rows ? 0 : (int64_t)(p.grid + 1) * 16 + 2 * (int64_t)p.grid * p.rows * slot_stride((int)c.head_dim) * 4;
 }
 
 template <typename T, int ROWS> void launch_join(const PagedArgs &a, int grid, cudaStream_t st) {
@@ -418,6 +419,7 @@ extern "C" int enc_paged_attention(const enc_paged_cache *cache, const enc_paged
     a.row_groups = p.row_groups; a.units = (int)cache->kv_heads * p.row_groups;
     a.whole = cache->page_size % 16 == 0;
     a.long_runs = p.long_runs;
+    a.by_rows = p.by_rows;
     a.scale = (float)(g.sm_scale * 1.4426950408889634);
     a.page_size = FastDiv((uint32_t)cache->page_size);
     cudaStream_t st = as_stream(stream);

@@ -14,6 +14,9 @@
 // two pieces of a run that belong to rows cut by its ends go to a workspace and a second, overlapped launch joins them in
 // order (no atomics: the result does not depend on timing).
 //
+// Where no row can have more than ROW_TILES tiles, rows are not cut at all: the line counts rows, and there is nothing to join
+// (one sequence of 130 keys: the same 10.5 us on the device, but 14.0 instead of 18.5 us a call from the host).
+//
 // Equal runs are not equal times: SMs differ by up to 1.3 in the bandwidth they get (measured per SM with equal runs: 500 to
 // 663 us at 48 x 32 kv heads).  So the runs come in two lengths: as many long ones as CTAs fit the GPU, 60% of the work, and
 // several times as many short ones that the tensor-core kernel's CTAs claim as they get free (680 -> 617 us).
@@ -27,6 +30,7 @@ namespace paged {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int TILE = 64;          // keys of a tile
+constexpr int ROW_TILES = 4;      // rows of at most so many tiles are not cut
 constexpr int MAX_HEAD_DIM = 256;
 
 struct PagedArgs {
@@ -41,6 +45,7 @@ struct PagedArgs {
     int64_t num_seqs, num_pages, capacity, window;
     int q_heads, head_dim, group, row_groups;  // query rows per kv head; row groups (of the kernel's row count) per kv head
     int units;                                 // row groups per sequence: kv_heads * row_groups
+    bool by_rows;                              // rows are not cut: the line counts row groups instead of tiles
     bool whole;                                // pages are whole multiples of 16 keys
     int long_runs;                             // runs of the first kind; the grid's other runs are short ones
     bool q_pairs;                              // query elements can be read two at a time
@@ -65,6 +70,8 @@ static __device__ __forceinline__ int keys_of(const PagedArgs &a, int64_t b, int
     return n - first;
 }
 static __device__ __forceinline__ int tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
+// What a sequence's row group takes up on the line: its tiles, or one where rows are not cut (a.by_rows).
+static __device__ __forceinline__ int weight_of(const PagedArgs &a, int keys) { return a.by_rows ? keys > 0 : tiles_of(keys); }
 
 // The line of tiles, as every CTA computes it (below 2^31 tiles: the host refuses more, and 32-bit divisions are several times
 // as fast as 64-bit ones).
@@ -108,7 +115,7 @@ static __device__ __forceinline__ Line make_line(const PagedArgs &a, int (&befor
     for (int64_t b = b0; b < b1; ++b) {
         const int keys = keys_of(a, b, first, skip);
         empty |= keys == 0;
-        mine += tiles_of(keys) * a.units;
+        mine += weight_of(a, keys) * a.units;
     }
     int upto = mine;
 #pragma unroll
@@ -148,7 +155,7 @@ static __device__ __forceinline__ void find_tile(const PagedArgs &a, const int (
     seq = piece * ((a.num_seqs + THREADS - 1) / THREADS);
     for (;; ++seq) {
         int first, skip;
-        const int t = tiles_of(keys_of(a, seq, first, skip)) * a.units;
+        const int t = weight_of(a, keys_of(a, seq, first, skip)) * a.units;
         if (at < t) return;
         at -= t;
     }
@@ -240,13 +247,14 @@ template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk
     if (pos < end) find_tile(a, before, pos, seq, at);
     while (pos < end) {
         int first, skip;
-        const int keys = keys_of(a, seq, first, skip), tiles = tiles_of(keys);
-        if (at >= tiles * a.units) {
-            at -= tiles * a.units;  // (zero: a sequence's tiles are walked to their end)
+        const int keys = keys_of(a, seq, first, skip), tiles = tiles_of(keys), weight = weight_of(a, keys);
+        if (at >= weight * a.units) {
+            at -= weight * a.units;  // (zero: a sequence is walked to its end)
             ++seq;
             continue;
         }
-        const int unit = at / tiles, t0 = at - unit * tiles, t1 = tiles - t0 < end - pos ? tiles : t0 + (end - pos);
+        const int unit = at / weight, t0 = at - unit * weight;  // (by rows: 0)
+        const int t1 = a.by_rows || tiles - t0 < end - pos ? tiles : t0 + (end - pos);
         const int kv_head = unit / a.row_groups, rg = unit - kv_head * a.row_groups;
         const int rows = a.group - rg * ROWS < ROWS ? a.group - rg * ROWS : ROWS;
         const int first_head = kv_head * a.group + rg * ROWS;
@@ -258,8 +266,8 @@ template <typename T, int ROWS, typename F> __device__ __forceinline__ void walk
             if (threadIdx.x == 0) a.headers[blockIdx.x] = make_int4((int)seq, rows | (first_head << 8), line.run_of(a, pos + tiles - 1), 0);
         }
         process(seq, kv_head, first_head, rows, first, skip, keys, t0, t1, slot);
-        pos += t1 - t0;
-        at += t1 - t0;
+        pos += a.by_rows ? 1 : t1 - t0;
+        at += a.by_rows ? 1 : t1 - t0;
     }
     if (line.any_empty) write_empty_rows<T>(a, blockIdx.x);
 }

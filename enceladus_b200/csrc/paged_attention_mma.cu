@@ -88,7 +88,7 @@ __device__ __forceinline__ int claimed(Claims &c, int i) {
 // A place in the CTA's runs: a tile of one unit (kv head and row group) of one sequence.
 struct Cursor {
     int64_t seq;
-    int left, end;           // tiles left in the run, the line's tile behind it
+    int left, end;           // tiles (by rows: row groups) left in the run, the line's tile behind it
     int run;                 // its number; -1: all done
     int unit, t, tiles, keys, first, skip;
 
@@ -105,14 +105,16 @@ struct Cursor {
         if (left <= 0) return;
         find_tile(a, before, begin, seq, at);
         read_keys(a);
-        unit = at / tiles;
-        t = at - unit * tiles;
+        const int weight = weight_of(a, keys);
+        unit = at / weight;
+        t = at - unit * weight;
     }
     // One tile on, inside the run.
     __device__ __forceinline__ void next(const PagedArgs &a) {
-        --left;
+        if (!a.by_rows) --left;
         if (++t < tiles) return;
         t = 0;
+        if (a.by_rows) --left;
         if (++unit < a.units || left <= 0) return;
         unit = 0;
         do {  // (left > 0: a sequence with keys follows)
@@ -466,8 +468,9 @@ template <typename T, int D, int STAGES, int CTAS, int NQ> int launch(PagedArgs 
     a.merge_rows = a.group < 8 * NQ ? a.group : 8 * NQ;
     a.merge_dims = R::TOTAL + WARPS * a.merge_rows * part_stride(D) * 4 <= budget(CTAS, NQ) ? D : D / 2;
     const int smem = R::TOTAL + WARPS * a.merge_rows * part_stride(a.merge_dims) * 4;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return fail(ENC_ERR_LAUNCH, "enc_paged_attention: cannot opt in to %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    static OncePerDevice opted[2];
+    const int rc = opted[a.whole].opt_in(kern, R::TOTAL + WARPS * 8 * NQ * part_stride(D) * 4, "enc_paged_attention");
+    if (rc != ENC_OK) return rc;
     launch_overlapped(kern, dim3(grid), dim3(THREADS), smem, st, a);
     return check_launch("enc_paged_attention");
 }

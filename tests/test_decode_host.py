@@ -22,7 +22,7 @@ def lib():
 
 
 def cache(**kw):
-    c = dict(k=16, v=16, block_table=16, num_pages=4, page_size=16, kv_heads=2, head_dim=64, num_seqs=3, table_width=5, stride_table=5,
+    c = dict(k=16, v=16, block_table=16, num_pages=4, page_size=16, kv_heads=2, head_dim=64, num_seqs=3, table_width=17, stride_table=17,
              k_stride_page=2048, k_stride_head=1024, k_stride_token=64, v_stride_page=2048, v_stride_head=1024, v_stride_token=64)
     c.update(kw)
     return N.paged_cache(*(c[n] or 0 for n in N.PAGED_CACHE_FIELDS))
@@ -112,7 +112,7 @@ def test_attention_refusals(lib):
     assert size > 0
     assert attend(lib, cache(), work=16, nbytes=size - 1) == bad and "workspace" in N.last_error()
     assert attend(lib, cache(), work=8, nbytes=size) == bad
-    assert lib.enc_paged_attention_work_bytes(cache(table_width=1), 4, N.F32, -1) == 0  # one tile per row: nothing is cut
+    assert lib.enc_paged_attention_work_bytes(cache(table_width=4), 4, N.F32, -1) == 0  # a tile per row: nothing is cut
     assert lib.enc_paged_attention_work_bytes(None, 4, N.F32, -1) == -1
     assert lib.enc_paged_attention_work_bytes(cache(), 3, N.F32, -1) == -1
 
