@@ -269,7 +269,8 @@ enum { V_TENSOR = 0, V_CORES = 1, VARIANTS = 2 };
 
 // The tensor-core kernels take 16-bit types, head dimensions they are instantiated for, and 16-byte rows in the cache.
 bool tensor_ok(const enc_paged_cache &c, int dtype) {
-    if (dtype_size(dtype) != 2 || mma_ctas_per_sm(c.head_dim) == 0 || !aligned16(c.k) || !aligned16(c.v)) return false;
+    // (an empty cache has no address that a copy could name)
+    if (dtype_size(dtype) != 2 || mma_ctas_per_sm(c.head_dim) == 0 || !c.k || !c.v || !aligned16(c.k) || !aligned16(c.v)) return false;
     for (int64_t s : {c.k_stride_page, c.k_stride_head, c.k_stride_token, c.v_stride_page, c.v_stride_head, c.v_stride_token})
         if (s % 8) return false;
     return true;

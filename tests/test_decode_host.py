@@ -205,3 +205,17 @@ def test_missing_arrays_are_refused_unless_optional(monkeypatch):
     assert ad.optional == frozenset(ad.array_list) - {"logits_ptr", "out_ptr"}
     soft = registry.lookup("softmax_kernel", tuple(ops.softmax_kernel.arg_names))
     assert not soft.optional
+
+
+def test_explain_names_the_entry_point_and_leaves_out_what_is_absent(lib, capsys):
+    f, _ = arrays()
+    x = f(2, 100)
+    text = ops.penalize_logits_kernel.explain(x, x, *[None] * 9, 100, 100, 100, 0, 0, 0, 0, 0, grid=(2,))
+    assert "enc_penalize_logits" in text and "logits_ptr" in text and "mask_ptr" not in text
+    assert "enc_paged_attention" in jit_entry("paged_attention_kernel") and "enc_append_kv" in jit_entry("append_kv_kernel")
+
+
+def jit_entry(name):
+    from enceladus_b200.runtime import jit
+
+    return jit._ENTRY_POINTS[getattr(ops, name).adapter().kernel_id]

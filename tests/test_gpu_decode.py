@@ -295,6 +295,41 @@ def test_attention_windows(dtype, window):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("page", [16, 24])
+def test_attention_what_lies_in_front_of_the_window_is_not_read(dtype, page):
+    """Pages that the window has left are gone from the table, and keys in front of it on its first page are NaN."""
+    lens, window = [500, 77, 16 * 20, 65], 70
+    for dim in (64, 128):
+        q, kc, vc, table = make_attention(dtype, lens, dim=dim, page=page, seed=dim)
+        o64, lse64, eo, el = attend64(q, kc, vc, table, lens, dim**-0.5, window)
+        for i, n in enumerate(lens):
+            lo = max(0, n - window)
+            at = int(table[i, lo // page])
+            kc[at, :, : lo % page] = math.nan
+            vc[at, :, : lo % page] = math.inf
+            table[i, : lo // page] = -1
+        o, lse = ops.paged_attention(q, kc, vc, table, ints(lens), window=window, return_lse=True)
+        enceladus.synchronize()
+        within(o, o64, half_step(dtype) * o64.abs() * (1 + 1e-6) + eo * 1.01 + TINY[dtype])
+        within(lse, lse64, el)
+
+
+def test_attention_over_an_empty_cache():
+    """No pages, or no columns: rows without keys are zero; a length that nothing can hold is cut and reported."""
+    for dtype in (BF16, F32):
+        q = randn(gen(8), 2, 4, 64, dtype=dtype)
+        for pages, columns in ((0, 3), (2, 0), (0, 0)):
+            kc = torch.zeros(pages, 2, 16, 64, device="cuda", dtype=dtype)
+            table = torch.zeros(2, columns, device="cuda", dtype=torch.int32)
+            o, lse = ops.paged_attention(q, kc, kc.clone(), table, ints([0, 0]), return_lse=True)
+            enceladus.synchronize()
+            assert not o.any() and (lse == -math.inf).all()
+            ops.paged_attention(q, kc, kc.clone(), table, ints([0, 5]))
+            with pytest.raises(enceladus.CudaError, match="out of range"):
+                enceladus.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
 def test_attention_long_rows_are_split(dtype):
     check_attention(dtype, [40_000], heads=(8, 1), dim=128, page=64, garbage=0.0)
     check_attention(dtype, [20_000, 3, 0, 9_999], heads=(4, 4), dim=64, page=32, garbage=0.0)
@@ -321,6 +356,31 @@ def test_attention_many_long_rows():
     lens = [int(x) for x in r.integers(1, 6000, 100)]
     check_attention(F16, lens, heads=(8, 8), dim=64, page=32, variants=False, garbage=0.0, extra=200, window=4000)
     check_attention(BF16, lens, heads=(36, 4), dim=64, page=24, variants=False, garbage=0.0, extra=200)
+
+
+def test_attention_large_launches_side_by_side():
+    """Launches large enough to claim runs from one another's blocks, on three streams at once and captured: the same bits."""
+    r = np.random.default_rng(2)
+    lens = [int(x) for x in r.integers(0, 3000, 160)]
+    q, kc, vc, table = make_attention(BF16, lens, heads=(16, 4), dim=64, page=16, garbage=0.0, extra=300)
+    n = ints(lens)
+    first = ops.paged_attention(q, kc, vc, table, n)
+    o64, _, eo, _ = attend64(q, kc, vc, table, lens, 0.125, 0)
+    within(first, o64, half_step(BF16) * o64.abs() * (1 + 1e-6) + eo * 1.01)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops.paged_attention(q, kc, vc, table, n)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(18):
+        with torch.cuda.stream(streams[i % 3]):
+            if i % 3 == 2:
+                graph.replay()
+            else:
+                got.append(ops.paged_attention(q, kc, vc, table, n))
+    torch.cuda.synchronize()
+    assert torch.equal(first, captured) and all(torch.equal(first, x) for x in got)
+    enceladus.synchronize()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
