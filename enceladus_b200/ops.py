@@ -315,7 +315,10 @@ def _check_cache(k_cache, v_cache, block_table):
                          f"{tuple(shape)} and {tuple(v_cache.shape)}")
     if len(block_table.shape) != 2:
         raise ValueError(f"block_table must have shape (sequences, pages per sequence), not {tuple(block_table.shape)}")
-    ks, vs, ts = _strides(k_cache), _strides(v_cache), _strides(block_table)
+    try:
+        ks, vs, ts = k_cache.stride(), v_cache.stride(), block_table.stride()
+    except AttributeError:
+        ks, vs, ts = _strides(k_cache), _strides(v_cache), _strides(block_table)
     if ks[3] != 1 or vs[3] != 1 or ts[1] != 1:
         for x, st, what in ((k_cache, ks, "k_cache"), (v_cache, vs, "v_cache"), (block_table, ts, "block_table")):
             if x.shape[-1] > 1 and st[-1] != 1 and 0 not in x.shape:
@@ -328,7 +331,10 @@ def _check_heads(x, what: str, rows: int, head_dim: int, heads: int | None = Non
     shape = x.shape
     if len(shape) != 3 or shape[0] != rows or shape[2] != head_dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what} must have shape ({rows}, {'heads' if heads is None else heads}, {head_dim}), not {tuple(shape)}")
-    st = _strides(x)
+    try:
+        st = x.stride()
+    except AttributeError:
+        st = enceladus.element_strides(x)
     if st[2] != 1 and head_dim > 1 and 0 not in shape:
         raise ValueError(f"the last dimension of {what} must be contiguous")
     return st
@@ -508,8 +514,11 @@ def penalize_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition
         if lens is None or prompt_lens is None or repetition is None or frequency is None or presence is None:
             raise ValueError("tokens, lens, prompt_lens, repetition, frequency and presence go together")
         stride_tokens, history = rows_of(tokens, "tokens"), tokens.shape[1]
-        for x, what in zip(past[1:], ("lens", "prompt_lens", "repetition", "frequency", "presence")):
-            _check_row(x, what, m)
+        _check_row(lens, "lens", m)
+        _check_row(prompt_lens, "prompt_lens", m)
+        _check_row(repetition, "repetition", m)
+        _check_row(frequency, "frequency", m)
+        _check_row(presence, "presence", m)
     elif any(x is not None for x in past):
         raise ValueError("tokens, lens, prompt_lens, repetition, frequency and presence go together")
     if (bias_ids is None) != (bias_values is None):

@@ -125,6 +125,9 @@ def dtype_code(obj: Any) -> int:
 
 
 def _new_array(like: Any, shape: Any, dtype: Any, zero: bool) -> Any:
+    if shape is None and dtype is None and not zero and _torch_mod is not None and isinstance(like, _torch_mod.Tensor) \
+            and like.is_contiguous() and like.dtype in _TORCH_NP:
+        return _torch_mod.empty_like(like)  # the commonest case, at half the cost of the general one
     shape = tuple(like.shape) if shape is None else tuple(shape)
     if isinstance(like, np.ndarray):
         dt = np.dtype(like.dtype if dtype is None else dtype)
