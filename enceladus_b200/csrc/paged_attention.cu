@@ -14,7 +14,7 @@ namespace {
 // of the CTA's headers side by side; rows cut into many (one long sequence has one per run) take the whole CTA, its warps
 // every JOIN_WARPS-th piece and then their results.  Lanes hold four neighbouring elements each; JOIN_DEEP pieces are in
 // flight per warp, because each is a trip to L2; one pass with a running maximum.
-constexpr int JOIN_WARPS = 8, JOIN_DEEP = 8, JOIN_FEW = 2 * JOIN_DEEP, JOIN_HEADERS = 64;
+constexpr int JOIN_WARPS = 8, JOIN_DEEP = 4, JOIN_FEW = 4 * JOIN_DEEP, JOIN_HEADERS = 64;
 
 struct Partial {
     float x[4], m, l;
@@ -59,7 +59,7 @@ template <typename T> __device__ __forceinline__ void write_row(const PagedArgs 
     if (d == 0 && a.lse) a.lse[seq * a.q_heads + head] = s.l == 0.0f ? -INFINITY : (s.m + log2f(s.l)) * LN2;
 }
 
-template <typename T, int ROWS> __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(PagedArgs a, int grid) {
+template <typename T, int ROWS> __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) join_kernel(PagedArgs a, int grid) {
     __shared__ int4 header[JOIN_HEADERS];
     __shared__ Partial parts[JOIN_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
