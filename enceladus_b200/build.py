@@ -4,6 +4,9 @@
 
 Each .cu file under csrc/ is compiled to an object (in parallel) and linked into
 enceladus_b200/lib/libenc_b200.so.  Objects are rebuilt when a source or header is newer.
+csrc/torch_lane.cpp, the short way from torch tensors to the decoding step's entry points, becomes
+enceladus_b200/lib/enc_torch_lane.so (host code only, g++ against torch's and Python's headers).  The library and
+its binding work without it, so a host without those headers gets a message instead of an error.
 """
 
 from __future__ import annotations
@@ -19,6 +22,7 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 LIBDIR = ROOT / "lib"
 LIB = LIBDIR / "libenc_b200.so"
+LANE = LIBDIR / "enc_torch_lane.so"
 OBJDIR = ROOT / "build"
 
 NVCC_FLAGS = [
@@ -46,7 +50,37 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def build_lane(force: bool = False, verbose: bool = False) -> Path | None:
+    """Builds the torch lane where it is older than its sources; None where that is not possible."""
+    import sysconfig
+    from importlib.util import find_spec
+
+    src = CSRC / "torch_lane.cpp"
+    newest = max(p.stat().st_mtime for p in (src, ROOT.parent / "include" / "enceladus_b200.h"))
+    if not force and LANE.exists() and LANE.stat().st_mtime >= newest:
+        return LANE
+    spec, cxx = find_spec("torch"), shutil.which("g++")
+    python_h = Path(sysconfig.get_paths()["include"])
+    if spec is None or cxx is None or not (python_h / "Python.h").exists():
+        sys.stderr.write("enc_torch_lane.so is not built (it needs g++, torch and Python's headers); calls go the longer way\n")
+        return None
+    torch, cuda = Path(spec.origin).parent, Path(nvcc()).resolve().parents[1]
+    LIBDIR.mkdir(exist_ok=True)
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{torch}/include", f"-I{torch}/include/torch/csrc/api/include",
+           f"-I{cuda}/include", f"-I{python_h}", str(src), "-o", str(LANE), f"-L{torch}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+    if r.returncode != 0:
+        LANE.unlink(missing_ok=True)  # none rather than a stale one
+        sys.stderr.write("enc_torch_lane.so could not be built; calls go the longer way\n")
+        return None
+    return LANE
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_lane(force, verbose)
     if not force and not needs_build():
         return LIB
     OBJDIR.mkdir(exist_ok=True)

@@ -11,13 +11,13 @@ A user's own copy of a reference example works the same way after `import encela
 from __future__ import annotations
 
 import math
-import os
 
 import numpy as np
 
 import enceladus_b200 as enceladus
 import enceladus_b200.language as tl
-from enceladus_b200.runtime import interop, registry
+from enceladus_b200 import _native as N
+from enceladus_b200.runtime import lane
 from enceladus_b200.configs import attention_configs, matmul_configs
 
 
@@ -284,9 +284,9 @@ def cumsum(x, reverse: bool = False):
 
 
 # ---- the decoding step: paged key-value cache, attention of one new token, logits -----------------------
-# A step runs once per generated token and its kernels can be as short as a few microseconds, so these wrappers keep the host's
-# share small: plain checks, and with torch tensors on the current device one call into the library without the launch path's
-# bookkeeping (`_straight`).  Everything else (NumPy arrays, another device, a forced variant) goes through `kernel[grid](...)`.
+# A step runs once per generated token and its kernels can be as short as a few microseconds.  So a call on torch tensors tries
+# the short way first (runtime/lane.py), which takes every valid call on the current device; what it does not take (NumPy arrays,
+# another device, a forced variant, empty or wrong arguments) is checked here and goes through `kernel[grid](...)`.
 def _strides(x):
     """Strides in elements."""
     try:
@@ -295,11 +295,15 @@ def _strides(x):
         return enceladus.element_strides(x)
 
 
-def _straight(kernel, *arrays) -> int | None:
-    """The stream for a straight call into the library, or None if the launch has to take the general path."""
-    if kernel.variant is not None or kernel.interpret is not None or "ENCELADUS_INTERPRET" in os.environ:
-        return None
-    return interop.direct_stream(*arrays)
+def _short(kernel, name: str, *args):
+    """The result of a call that went the short way, or NotImplemented."""
+    way = lane.get()
+    if way is None or kernel.variant is not None or kernel.interpret is not None:
+        return NotImplemented
+    r = getattr(way, name)(*args)
+    if type(r) is int:  # an enc_status: raises
+        N.check(r)
+    return r
 
 
 def _no_overlap(x, st, what: str) -> None:
@@ -315,10 +319,7 @@ def _check_cache(k_cache, v_cache, block_table):
                          f"{tuple(shape)} and {tuple(v_cache.shape)}")
     if len(block_table.shape) != 2:
         raise ValueError(f"block_table must have shape (sequences, pages per sequence), not {tuple(block_table.shape)}")
-    try:
-        ks, vs, ts = k_cache.stride(), v_cache.stride(), block_table.stride()
-    except AttributeError:
-        ks, vs, ts = _strides(k_cache), _strides(v_cache), _strides(block_table)
+    ks, vs, ts = _strides(k_cache), _strides(v_cache), _strides(block_table)
     if ks[3] != 1 or vs[3] != 1 or ts[1] != 1:
         for x, st, what in ((k_cache, ks, "k_cache"), (v_cache, vs, "v_cache"), (block_table, ts, "block_table")):
             if x.shape[-1] > 1 and st[-1] != 1 and 0 not in x.shape:
@@ -331,10 +332,7 @@ def _check_heads(x, what: str, rows: int, head_dim: int, heads: int | None = Non
     shape = x.shape
     if len(shape) != 3 or shape[0] != rows or shape[2] != head_dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what} must have shape ({rows}, {'heads' if heads is None else heads}, {head_dim}), not {tuple(shape)}")
-    try:
-        st = x.stride()
-    except AttributeError:
-        st = enceladus.element_strides(x)
+    st = _strides(x)
     if st[2] != 1 and head_dim > 1 and 0 not in shape:
         raise ValueError(f"the last dimension of {what} must be contiguous")
     return st
@@ -373,6 +371,9 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_ids, positions, cos=None,
     turns. `q_out` may be `q`. A sequence, position or page out of range is skipped, and `synchronize()` raises
     `CudaError`.
     """
+    r = _short(append_kv_kernel, "append_kv", k, v, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, q, q_out, interleaved)
+    if r is not NotImplemented:
+        return r
     ks, vs, st = _check_cache(k_cache, v_cache, block_table)
     pages, kv_heads, page_size, d = k_cache.shape
     tokens = k.shape[0]
@@ -406,12 +407,6 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_ids, positions, cos=None,
         if not rot_dim:
             cos = sin = None
     seqs, width = block_table.shape
-    stream = _straight(append_kv_kernel, k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin)
-    if stream is not None:
-        registry.append_kv(k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, tokens, seqs, width, st, pages,
-                           n_positions, k_st, v_st, q_st, o_st, cos_st, ks, vs, q_heads, kv_heads, d, rot_dim,
-                           page_size, 1 if interleaved else 0, -1, stream)
-        return q_out
     append_kv_kernel[(tokens,)](k, v, q, q_out, k_cache, v_cache, block_table, seq_ids, positions, cos, sin, seqs, width, st, pages,
                                 n_positions, k_st[0], k_st[1], v_st[0], v_st[1], q_st[0], q_st[1],
                                 o_st[0], o_st[1], cos_st, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,
@@ -441,6 +436,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale: float 
     With `return_lse=True`, also returns the float32 log-sum-exp of the scaled scores, shape (sequences, q_heads):
     -inf for a row without keys. A length or page out of range is cut or skipped, and `synchronize()` raises `CudaError`.
     """
+    r = _short(paged_attention_kernel, "paged_attention", q, k_cache, v_cache, block_table, seq_lens, sm_scale, window, o, return_lse)
+    if r is not NotImplemented:
+        return r
     ks, vs, st = _check_cache(k_cache, v_cache, block_table)
     pages, kv_heads, page_size, d = k_cache.shape
     seqs = q.shape[0]
@@ -461,11 +459,6 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale: float 
     _no_overlap(o, o_st, "o")
     scale = 1.0 / math.sqrt(d) if sm_scale is None else sm_scale
     lse = enceladus.new_empty(q, (seqs, q_heads), np.float32) if return_lse else None
-    stream = _straight(paged_attention_kernel, q, k_cache, v_cache, o, lse, block_table, seq_lens)
-    if stream is not None:
-        registry.paged_attention(q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, seqs, block_table.shape[1], st, pages,
-                                 q_st, o_st, ks, vs, q_heads, kv_heads, d, page_size, -1, stream)
-        return (o, lse) if return_lse else o
     paged_attention_kernel[(seqs,)](q, k_cache, v_cache, o, lse, block_table, seq_lens, scale, window, block_table.shape[1], st, pages,
                                     q_st[0], q_st[1], o_st[0], o_st[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Q_HEADS=q_heads,
                                     KV_HEADS=kv_heads, HEAD_DIM=d, PAGE_SIZE=page_size)
@@ -494,6 +487,10 @@ def penalize_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition
     The history's arrays come together, the biases' too, and each part can be left out. `out` may be `logits`.
     A token, bias id or length out of range is ignored or cut, and `synchronize()` raises `CudaError`.
     """
+    r = _short(penalize_logits_kernel, "penalize_logits", logits, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values,
+               mask, out)
+    if r is not NotImplemented:
+        return r
     if len(logits.shape) != 2:
         raise ValueError(f"logits must have shape (rows, vocab), not {tuple(logits.shape)}")
     m, n = logits.shape
@@ -535,11 +532,6 @@ def penalize_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition
         out = enceladus.new_empty(logits)
     so = rows_of(out, "out", n)
     _no_overlap(out, (so,), "out")
-    stream = _straight(penalize_logits_kernel, logits, out, *past, bias_ids, bias_values, mask)
-    if stream is not None and m:
-        registry.penalize_logits(logits, out, *past, bias_ids, bias_values, mask, m, n, si, so, history, stride_tokens, n_biases, stride_bias,
-                                 stride_mask, -1, stream)
-        return out
     penalize_logits_kernel[(m,)](logits, out, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, mask,
                                  n, si, so, history, stride_tokens, n_biases, stride_bias, stride_mask)
     return out

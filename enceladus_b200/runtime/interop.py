@@ -200,23 +200,6 @@ def current_stream() -> int:
     return raw(torch.cuda.current_device()) if raw is not None else int(torch.cuda.current_stream().cuda_stream)
 
 
-def direct_stream(*arrays: Any) -> int | None:
-    """The current stream if a launch over these arrays can go straight to the library: every array (None: left out) is a
-    torch tensor on the current CUDA device, so there is nothing to stage and no device to switch.  None otherwise."""
-    torch = _torch_mod
-    if torch is None or not torch.cuda.is_initialized():
-        return None
-    dev = torch.cuda.current_device()
-    try:
-        for a in arrays:
-            if a is not None and a.get_device() != dev:  # (-1: in host memory)
-                return None
-    except AttributeError:  # a NumPy array, or no array at all
-        return None
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(dev) if raw is not None else current_stream()
-
-
 def _np_as_torch_view(a: np.ndarray):
     """A torch CPU tensor sharing the memory of a NumPy array (bfloat16 through its uint16 bits)."""
     torch = _torch()

@@ -346,8 +346,7 @@ def _attention_lse(a, grid, variant, stream):
 
 
 # ---- the decoding step: paged cache, attention of one new token, logits -----------------------------
-# Each of the three calls below takes device tensors and sizes; the launch path reaches it through the adapter under it, the
-# wrapper in ops.py directly when there is nothing to stage.
+# Each of the three calls below takes device tensors and sizes, and is followed by the adapter that reads them out of a launch.
 def _opt(t: Any) -> int:
     return 0 if t is None else t.data_ptr()
 

@@ -705,6 +705,90 @@ def test_numpy_arguments():
     assert np.array_equal(y, y2.cpu().numpy())
 
 
+def general(kernel):
+    """The kernel's calls go through `kernel[grid](...)` while this is in force."""
+    class Way:
+        def __enter__(self):
+            kernel.variant = N.VARIANT_AUTO
+
+        def __exit__(self, *_):
+            kernel.variant = None
+
+    return Way()
+
+
+def test_the_short_way_and_the_launch_path_agree():
+    """Every valid call on device tensors goes the short way, with the launch path's bits; nothing else does."""
+    from enceladus_b200.runtime import lane
+
+    way = lane.get()
+    assert way is not None, "enc_torch_lane.so is not built"
+    g = gen(9)
+    for dtype in (BF16, F16, F32):
+        q, kc, vc, table = make_attention(dtype, [300, 0, 41], dim=64, garbage=0.0)
+        n = ints([300, 0, 41])
+        for scale, window in ((None, 0), (0.3, 100), (1, 2**40)):
+            args = (q, kc, vc, table, n, scale, window, None, True)
+            assert way.paged_attention(*args) is not NotImplemented
+            a = ops.paged_attention(q, kc, vc, table, n, sm_scale=scale, window=window, return_lse=True)
+            with general(ops.paged_attention_kernel):
+                b = ops.paged_attention(q, kc, vc, table, n, sm_scale=scale, window=window, return_lse=True)
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        k, v, cos, sin = randn(g, 3, 2, 64, dtype=dtype), randn(g, 3, 2, 64, dtype=dtype), *tables(400, 48)
+        ids, pos = ints([0, -1, 2]), ints([299, 0, 40])
+        for interleaved in (False, True):
+            for rot in ((cos, sin), (None, None)):
+                caches = [kc.clone(), vc.clone()], [kc.clone(), vc.clone()]
+                outs = [torch.zeros_like(q) for _ in range(2)]
+                assert way.append_kv(k, v, *caches[0], table, ids, pos, *rot, q, outs[0], interleaved) is outs[0]
+                with general(ops.append_kv_kernel):
+                    assert ops.append_kv(k, v, *caches[1], table, ids, pos, *rot, q=q, q_out=outs[1], interleaved=interleaved) is outs[1]
+                assert torch.equal(outs[0], outs[1]) and all(torch.equal(x, y) for x, y in zip(*caches))
+        assert way.append_kv(k, v, kc, vc, table, ids, pos, None, None, None, None, False) is None
+        x, *rest = make_logits(dtype, 3, 777, 50, 5, True)
+        for parts in (rest, [*rest[:6], None, None, None], [None] * 6 + rest[6:], [None] * 9):
+            assert way.penalize_logits(x, *parts, None) is not NotImplemented
+            names = ("tokens", "lens", "prompt_lens", "repetition", "frequency", "presence", "bias_ids", "bias_values", "mask")
+            a = ops.penalize_logits(x, **dict(zip(names, parts)))
+            with general(ops.penalize_logits_kernel):
+                b = ops.penalize_logits(x, **dict(zip(names, parts)))
+            assert torch.equal(a, b)
+        enceladus.synchronize()
+
+        bad_k = k.double()
+        for args in ((bad_k, v, kc, vc, table, ids, pos), (k, v[:2], kc, vc, table, ids, pos), (k, v, kc, vc[:1], table, ids, pos),
+                     (k, v, kc, vc, table.long(), ids, pos), (k, v, kc, vc, table, ids.long(), pos), (k, v, kc, vc, table, ids, pos[:2]),
+                     (k.cpu(), v, kc, vc, table, ids, pos), (k, v, kc[:1].expand_as(kc), vc, table, ids, pos), (k, v, kc.transpose(2, 3), vc, table, ids, pos),
+                     (None, v, kc, vc, table, ids, pos), (k.cpu().float().numpy(), v, kc, vc, table, ids, pos), (k[:0], v[:0], kc, vc, table, ids[:0], pos[:0])):
+            assert way.append_kv(*args, cos, sin, None, None, False) is NotImplemented
+        for extra in ((cos, None, q, None), (cos.double(), sin.double(), q, None), (cos[:, ::2], sin[:, ::2], q, None), (cos, sin, None, q), (cos, sin, q, q[:2]),
+                      (cos, sin, q, q[:, :1].expand_as(q)), (*tables(9, 66), q, None)):
+            assert way.append_kv(k, v, kc, vc, table, ids, pos, *extra, False) is NotImplemented
+        for args in ((q[:, :3], kc, vc, table, n), (q[:2], kc, vc, table, n), (q, kc, vc, table[:2], n), (q, kc, vc, table, n.long()), (q, kc, vc, table, n[:2]),
+                     (q.cpu(), kc, vc, table, n), (q.transpose(0, 1), kc, vc, table, n), (q[..., :32], kc, vc, table, n)):
+            assert way.paged_attention(*args, None, 0, None, False) is NotImplemented
+        for extra in (("x", 0, None, False), (None, -1, None, False), (None, 1.5, None, False), (None, 2**70, None, False), (None, 0, q[:2], False)):
+            assert way.paged_attention(q, kc, vc, table, n, *extra) is NotImplemented
+        assert way.penalize_logits(x, *rest[:5], None, *rest[6:], None) is NotImplemented
+        assert way.penalize_logits(x, None, *rest[1:], None) is NotImplemented
+        assert way.penalize_logits(x, *rest[:8], rest[8][:, 1:], None) is NotImplemented
+        assert way.penalize_logits(x, *rest, x[:, :5]) is NotImplemented
+        assert way.penalize_logits(x.t(), *[None] * 10) is NotImplemented
+        assert way.penalize_logits(x) is NotImplemented
+    with pytest.raises(ValueError, match="go together"):
+        ops.penalize_logits(x, *rest[:5])
+    with pytest.raises(TypeError, match="must be int32"):
+        ops.paged_attention(q, kc, vc, table, n.long())
+    lib = N.load()
+    lib.enc_test_fail_next(N.ERR_LAUNCH)
+    with pytest.raises(enceladus.CudaError, match="injected"):
+        ops.paged_attention(q, kc, vc, table, n)
+    with pytest.raises(NotImplementedError, match="head_dim"):  # an error of the library's own, worded there
+        with general(ops.paged_attention_kernel):
+            ops.paged_attention_kernel[(1,)](q, kc, vc, q, None, table, n, 1.0, 0, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, Q_HEADS=2, KV_HEADS=2,
+                                             HEAD_DIM=300, PAGE_SIZE=16)
+
+
 def decode_step(w, x, kc, vc, table, ids, pos, lens, cos, sin, past, mask):
     """One layer and a head, made of the framework's operators only."""
     b, hid = x.shape
