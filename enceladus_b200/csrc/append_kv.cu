@@ -68,12 +68,16 @@ template <typename T, int N> struct Elems<T, N, true> {
     __device__ __forceinline__ void set(const float (&f)[N]) { v = Pack<T>::pack(f); }
 };
 
+// Bytes in flight are what a CTA's short life is about, so registers are capped for as many CTAs as that leaves without spills
+// (5016 float32 tokens of 18 heads of 64, pairs of neighbours: 15.0 us at 8 CTAs per SM, 12.7 at 12).
+template <typename T, bool INTERLEAVED> constexpr int append_ctas_per_sm() { return sizeof(T) == 4 ? (INTERLEAVED ? 12 : 10) : 8; }
+
 // One CTA per token.  VEC: 16-byte vectors (NV elements); else single elements.  An item is one place inside a head: a pair
 // of vectors that turn together (one vector of neighbouring pairs when INTERLEAVED), or a vector that is copied.  The loads
 // of a thread's first UN heads and of its first value vector are under way before the token's position, its page and its
 // angles have arrived: they are the longest chain (index -> page number, position -> cosines).
 template <typename T, bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(THREADS, 8) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(THREADS, append_ctas_per_sm<T, INTERLEAVED>()) append_kernel(AppendArgs a) {
     constexpr int NV = VEC ? Pack<T>::N : (INTERLEAVED ? 2 : 1);  // elements of an item's vector
     constexpr int UN = 3;                                         // heads in flight per thread
     constexpr int NC = INTERLEAVED ? NV / 2 : NV;                 // angles of an item
