@@ -265,14 +265,14 @@ template <typename T, int CH, int ROWS, bool VEC> __global__ void __launch_bound
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-enum { V_TENSOR = 0, V_CORES = 1, VARIANTS = 2 };
+enum { V_RING = 0, V_CORES = 1, VARIANTS = 2 };
 
-// The tensor-core kernels take 16-bit types, head dimensions they are instantiated for, and 16-byte rows in the cache.
-bool tensor_ok(const enc_paged_cache &c, int dtype) {
+// The ring kernels take the head dimensions they are instantiated for, and 16-byte rows in the cache.
+bool ring_ok(const enc_paged_cache &c, int dtype) {
     // (an empty cache has no address that a copy could name)
-    if (dtype_size(dtype) != 2 || mma_ctas_per_sm(c.head_dim) == 0 || !c.k || !c.v || !aligned16(c.k) || !aligned16(c.v)) return false;
+    if (ring_ctas_per_sm(dtype, c.head_dim) == 0 || !c.k || !c.v || !aligned16(c.k) || !aligned16(c.v)) return false;
     for (int64_t s : {c.k_stride_page, c.k_stride_head, c.k_stride_token, c.v_stride_page, c.v_stride_head, c.v_stride_token})
-        if (s % 8) return false;
+        if (s % (16 / (int64_t)dtype_size(dtype))) return false;
     return true;
 }
 
@@ -285,10 +285,10 @@ struct Plan {
 // Which kernel, how many query rows it takes at a time, how many CTAs, and the bytes for pieces.
 void make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant, Plan &p) {
     const int group = (int)(q_heads / c.kv_heads);
-    p.variant = variant >= 0 ? variant : tensor_ok(c, dtype) ? V_TENSOR : V_CORES;
-    p.rows = p.variant == V_TENSOR ? mma_rows(group) : group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
+    p.variant = variant >= 0 ? variant : ring_ok(c, dtype) ? V_RING : V_CORES;
+    p.rows = p.variant == V_RING ? ring_rows(dtype, group) : group == 1 ? 1 : c.head_dim > 128 ? 2 : 4;
     const int ch = c.head_dim > 128 ? 8 : c.head_dim > 64 ? 4 : 2;
-    const int per_sm = p.variant == V_TENSOR ? mma_ctas_per_sm(c.head_dim) : cores_ctas_per_sm(ch, p.rows);
+    const int per_sm = p.variant == V_RING ? ring_ctas_per_sm(dtype, c.head_dim) : cores_ctas_per_sm(ch, p.rows);
     p.row_groups = (int)cdiv(group, p.rows);
     const int64_t units = c.num_seqs * c.kv_heads * p.row_groups, row_tiles = cdiv(paged_capacity(c), TILE);
     p.by_rows = row_tiles <= ROW_TILES;
@@ -298,7 +298,7 @@ void make_plan(const enc_paged_cache &c, int64_t q_heads, int dtype, int variant
     // Short runs even out the SMs (see paged_attention.cuh) but cost two microseconds each: measured at 48 x 32 kv heads (664
     // tiles a CTA at most) 685 us without, 637 with two per long run, 618 with six; at 64 x 8 (110 tiles) 105, 102, 140.  With
     // fewer rows than CTAs every short run is a piece that the join has to fetch (2 x 4: 101 us without, 120 with two).
-    const int shorts = p.variant != V_TENSOR || p.by_rows || units < fill || most < 64 * fill ? 0 : most < 256 * fill ? 2 : 6;
+    const int shorts = p.variant != V_RING || p.by_rows || units < fill || most < 64 * fill ? 0 : most < 256 * fill ? 2 : 6;
     p.grid = p.long_runs * (1 + shorts);
     p.work = p.by_rows ? 0 : (int64_t)(p.grid + 1) * 16 + 2 * (int64_t)p.grid * p.rows * slot_stride((int)c.head_dim) * 4;
 }
@@ -320,14 +320,18 @@ void launch_simple(const PagedArgs &a, int grid, bool vec, cudaStream_t st) {
 
 template <typename T> int launch_paged(const PagedArgs &a, const Plan &p, cudaStream_t st) {
     note_indexed_launch();
-    if constexpr (sizeof(T) == 2) {
-        if (p.variant == V_TENSOR) {
-            const int rc = launch_mma(a, std::is_same<T, __half>::value ? ENC_F16 : ENC_BF16, p.grid, st);
-            if (rc != ENC_OK) return rc;
+    if (p.variant == V_RING) {
+        const int dtype = std::is_same<T, float>::value ? ENC_F32 : std::is_same<T, __half>::value ? ENC_F16 : ENC_BF16;
+        const int rc = launch_ring(a, dtype, p.grid, st);
+        if (rc != ENC_OK) return rc;
+        if constexpr (sizeof(T) == 4) {
+            if (p.rows == 1) launch_join<T, 1>(a, p.grid, st);
+            else launch_join<T, 4>(a, p.grid, st);
+        } else {
             if (p.rows == 8) launch_join<T, 8>(a, p.grid, st);
             else launch_join<T, 16>(a, p.grid, st);
-            return check_launch("enc_paged_attention");
         }
+        return check_launch("enc_paged_attention");
     }
     const int nv = 4;
     bool vec = a.head_dim % nv == 0;
@@ -358,18 +362,18 @@ int check_paged(const enc_paged_cache *c, int64_t q_heads, int dtype, int varian
     if ((double)c->num_seqs * (double)q_heads * (double)cdiv(paged_capacity(*c), TILE) >= 2147400000.0)  // (room for a run more)
         return fail(ENC_ERR_UNSUPPORTED, "%s: %lld sequences of up to %lld keys with %lld heads pass 2^31 tiles of %d keys", me,
                     (long long)c->num_seqs, (long long)paged_capacity(*c), (long long)q_heads, TILE);
-    if (variant == V_TENSOR && !tensor_ok(*c, dtype))
-        return fail(ENC_ERR_UNSUPPORTED, "%s: variant %d needs float16 or bfloat16, another head_dim, or 16-byte aligned cache rows", me, variant);
+    if (variant == V_RING && !ring_ok(*c, dtype))
+        return fail(ENC_ERR_UNSUPPORTED, "%s: variant %d needs another head_dim, or 16-byte aligned cache rows", me, variant);
     return 0;
 }
 
 }  // namespace
 
-unsigned int take_bad_index_paged_mma();
-unsigned int take_bad_index_paged_attention() { return take_bad_index_word() | take_bad_index_paged_mma(); }
+unsigned int take_bad_index_paged_ring();
+unsigned int take_bad_index_paged_attention() { return take_bad_index_word() | take_bad_index_paged_ring(); }
 int paged_attention_variants() { return VARIANTS; }
 void paged_attention_variant_info(int v, char *out, size_t n) {
-    if (v == V_TENSOR) snprintf(out, n, "mma m16n8k16, 16 keys by 8 or 16 query rows per warp and step, keys and values through a cp.async ring");
+    if (v == V_RING) snprintf(out, n, "keys and values through a cp.async ring per warp, 16 keys a step; 16-bit types by mma m16n8k16, float32 on CUDA cores");
     else snprintf(out, n, "CUDA cores, eight lanes per key, keys and values straight to registers");
 }
 
@@ -380,7 +384,7 @@ extern "C" int64_t enc_paged_attention_work_bytes(const enc_paged_cache *cache, 
     if (check_paged(cache, q_heads, dtype, variant < 0 ? -1 : V_CORES, "enc_paged_attention_work_bytes") || variant >= VARIANTS) return -1;
     int64_t most = 0;
     for (int v = 0; v < VARIANTS; ++v) {
-        if ((variant >= 0 && v != variant) || (v == V_TENSOR && (dtype_size(dtype) != 2 || mma_ctas_per_sm(cache->head_dim) == 0))) continue;
+        if ((variant >= 0 && v != variant) || (v == V_RING && ring_ctas_per_sm(dtype, cache->head_dim) == 0)) continue;
         Plan p;
         make_plan(*cache, q_heads, dtype, v, p);
         if (p.work > most) most = p.work;

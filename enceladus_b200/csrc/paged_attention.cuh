@@ -19,7 +19,7 @@
 //
 // Equal runs are not equal times: SMs differ by up to 1.3 in the bandwidth they get (measured per SM with equal runs: 500 to
 // 663 us at 48 x 32 kv heads).  So the runs come in two lengths: as many long ones as CTAs fit the GPU, 60% of the work, and
-// several times as many short ones that the tensor-core kernel's CTAs claim as they get free (680 -> 617 us).
+// several times as many short ones that the ring kernel's CTAs claim as they get free (680 -> 617 us).
 #pragma once
 
 #include "paged.cuh"
@@ -283,10 +283,11 @@ static __device__ __forceinline__ bool locate(const PagedArgs &a, int64_t seq, i
 }
 
 
-// Tensor-core kernels (paged_attention_mma.cu): whether there is one for this head_dim, CTAs per SM, and the launch.
-int mma_ctas_per_sm(int64_t head_dim);                       // 0: none
-inline int mma_rows(int group) { return group <= 8 ? 8 : 16; }  // query rows that a CTA takes at a time
-int launch_mma(const PagedArgs &a, int dtype, int grid, cudaStream_t st);
+// The ring kernels (paged_attention_ring.cu): CTAs per SM for a type and head_dim, 0 where there is none, the query rows that a
+// CTA takes at a time, and the launch.
+int ring_ctas_per_sm(int dtype, int64_t head_dim);
+inline int ring_rows(int dtype, int group) { return dtype == ENC_F32 ? (group == 1 ? 1 : 4) : group <= 8 ? 8 : 16; }
+int launch_ring(const PagedArgs &a, int dtype, int grid, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace enc
