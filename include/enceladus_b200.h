@@ -15,6 +15,8 @@
  *   - the caller owns all buffers.  The library itself owns, per device: a 256-byte status block (bounded
  *     device-side waits report there) and the tile-descriptor scratch of enc_cumsum / enc_sum (see
  *     enc_cumsum); both are allocated on first use and freed at exit.  No other entry point allocates;
+ *   - index arrays (lengths, positions, pages, tokens of the decoding step) are device data, so they are checked on the device:
+ *     what they name out of range is skipped, and the next enc_synchronize on the device returns ENC_ERR_BAD_INDEX;
  *   - `stream` is a cudaStream_t / CUstream passed as void* (NULL = the legacy default stream); work
  *     is enqueued and the call returns without synchronising, like fr_stream_dispatch;
  *   - the return value is an enc_status; on failure enc_last_error() holds a message for the calling
