@@ -12,7 +12,8 @@
 // matter) and lists each token when it is first counted; the list is worked off over what was streamed and is still in L2.
 // Nothing the size of the vocabulary besides the logits touches memory.
 // Measured at 256 x 131072 float32 with histories up to 8192: penalties inside the stream 145 us, the list before the stream 131,
-// after it 102.  A second launch with a hash table per row 98 (its scattered reads and writes go to memory again), a cluster per
+// after it 102, queue and list 85 (of which the stream alone is 39).  A fourth CTA per SM (counts of 16 bits, 32 registers a
+// thread) 87.  A second launch with a hash table per row 98 (its scattered reads and writes go to memory again), a cluster per
 // row that counts each token once over distributed shared memory 235 (common tokens queue up at one CTA).
 #include <type_traits>
 
