@@ -61,10 +61,14 @@ def build_lane(force: bool = False, verbose: bool = False) -> Path | None:
         return LANE
     spec, cxx = find_spec("torch"), shutil.which("g++")
     python_h = Path(sysconfig.get_paths()["include"])
-    if spec is None or cxx is None or not (python_h / "Python.h").exists():
-        sys.stderr.write("enc_torch_lane.so is not built (it needs g++, torch and Python's headers); calls go the longer way\n")
+    try:
+        cuda = Path(nvcc()).resolve().parents[1]
+    except RuntimeError:
+        cuda = None
+    if spec is None or cxx is None or cuda is None or not (python_h / "Python.h").exists():
+        sys.stderr.write("enc_torch_lane.so is not built (it needs g++, the CUDA toolkit, torch and Python's headers); calls go the longer way\n")
         return None
-    torch, cuda = Path(spec.origin).parent, Path(nvcc()).resolve().parents[1]
+    torch = Path(spec.origin).parent
     LIBDIR.mkdir(exist_ok=True)
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{torch}/include", f"-I{torch}/include/torch/csrc/api/include",
            f"-I{cuda}/include", f"-I{python_h}", str(src), "-o", str(LANE), f"-L{torch}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu",

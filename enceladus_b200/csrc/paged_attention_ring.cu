@@ -480,7 +480,7 @@ template <typename T, int D, int STAGES, int CTAS, typename Math, bool WHOLE> __
         const int j = load.t * TILE + warp * 16 + (WHOLE ? 0 : lane & 15);
         if (j < load.keys) page = a.block_table[load.seq * a.s_table + a.page_size.div((uint32_t)(load.first + j))];
     };
-    auto issue = [&](int stage) {  // the copies of one tile's 16 keys and values, then one step on
+    auto issue = [&](int stage, bool ahead) {  // the copies of one tile's 16 keys and values, then one step on
         if (load.run >= 0) {
             const int j0 = load.t * TILE + warp * 16, n = load.keys - j0;  // keys of the 16 that exist
             const int kv_head = a.row_groups == 1 ? load.unit : load.unit / a.row_groups;
@@ -529,7 +529,7 @@ template <typename T, int D, int STAGES, int CTAS, typename Math, bool WHOLE> __
             }
             load.next(a);
             if (load.left <= 0) next_run();
-            read_page();
+            if (ahead) read_page();
         }
         cp_async_commit();
     };
@@ -549,9 +549,23 @@ template <typename T, int D, int STAGES, int CTAS, typename Math, bool WHOLE> __
     for (bool prime = true;;) {
         if (prime) {  // fill the ring
             prime = false;
-            read_page();
+            // One tile after the other would wait for one page number after the other: lane s asks for that of the s-th tile from
+            // here, as far as they are the same run's and sequence's (WHOLE: a warp needs one number a tile).
+            int early = 0, known = 0;
+            if (WHOLE && load.run >= 0) {
+                const int t = load.t + lane, ahead = t / load.tiles, j = (t - ahead * load.tiles) * TILE + warp * 16;
+                const bool same = lane < STAGES && (a.by_rows ? ahead < load.left : lane < load.left) && load.unit + ahead < a.units;
+                if (same && j < load.keys) early = a.block_table[load.seq * a.s_table + a.page_size.div((uint32_t)(load.first + j))];
+                known = __popc(__ballot_sync(0xffffffffu, same));
+            }
 #pragma unroll 1
-            for (int s = 0; s < STAGES; ++s) issue(stage + s < STAGES ? stage + s : stage + s - STAGES);
+            for (int s = 0; s < STAGES; ++s) {
+                const int number = __shfl_sync(0xffffffffu, early, s);
+                if (s < known) page = number;
+                else if (s == known) read_page();
+                issue(stage + s < STAGES ? stage + s : stage + s - STAGES, s >= known);
+            }
+            if (known >= STAGES) read_page();
         }
         if (at.run < 0) {
             // Runs without tiles are at the queue's end and wait for nothing; taken off it, a bounded number by each CTA, they
@@ -574,7 +588,7 @@ template <typename T, int D, int STAGES, int CTAS, typename Math, bool WHOLE> __
             math.step(a, ks, vs, left, WHOLE && at.t == 0 && warp == 0 ? at.skip : 0);
         }
         __syncwarp();
-        issue(stage);
+        issue(stage, true);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
 
         const int t1 = at.t + 1, tiles = at.tiles, run = at.run;
