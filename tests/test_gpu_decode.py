@@ -717,6 +717,47 @@ def general(kernel):
     return Way()
 
 
+def test_a_process_may_begin_with_a_captured_step():
+    """Nothing has to run before the first capture: no allocation, no set-up that a capture would refuse."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from enceladus_b200 import ops
+import enceladus_b200 as enceladus
+z = lambda *s, t=torch.bfloat16: torch.ones(*s, device="cuda", dtype=t)
+kc, vc, k, v, q, qo = z(400, 4, 16, 128), z(400, 4, 16, 128), z(8, 4, 128), z(8, 4, 128), z(8, 16, 128), z(8, 16, 128)
+kc2, q2 = z(400, 4, 16, 64, t=torch.float32), z(8, 4, 64, t=torch.float32)
+i = lambda x: x.to(torch.int32)
+table = i(torch.arange(400, device="cuda").reshape(8, 50))
+ids, pos, lens, x = i(torch.arange(8, device="cuda")), i(z(8) * 699), i(z(8) * 700), z(8, 50000)
+tok, one = i(z(8, 40)), z(8, t=torch.float32)
+cos = z(800, 64, t=torch.float32)
+out = torch.empty_like(x)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.append_kv(k * 3, v * 3, kc, vc, table, ids, pos, cos=cos, sin=cos * 0, q=q, q_out=qo)
+    o = ops.paged_attention(qo, kc, vc, table, lens)
+    o2 = ops.paged_attention(q2, kc2, kc2, table, lens)
+    o3 = ops.paged_attention(qo, kc, vc, table, lens + 1)
+    ops.penalize_logits(x, tok, ids * 0 + 40, ids * 0, one * 2, one, one, out=out)
+graph.replay()
+enceladus.synchronize()
+# 699 is 700 in bfloat16 (steps of 4): the new token lies in page 43, slot 12, the first behind the length
+assert (pos == 700).all() and (kc[table[:, 43].long(), :, 12] == 3).all() and (kc == 3).sum() == 8 * 4 * 128
+# without it every value is 1: a mean of ones, whose two sums of 700 and whose division round in float32
+assert (o == 1).all() and ((o2 - 1).abs() <= (2 * 700 + 4) * 2.0 ** -24).all(), (o, o2)
+# with it its score leads by 2 * 128 / sqrt(128) = 22.6, and the 700 ones move the result by 2e-7 from 3
+assert (o3 == 3).all(), o3
+assert (out[:, 1] == 0.5 - 41).all() and (out[:, 2:] == 1).all()
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_the_short_way_and_the_launch_path_agree():
     """Every valid call on device tensors goes the short way, with the launch path's bits; nothing else does."""
     from enceladus_b200.runtime import lane
