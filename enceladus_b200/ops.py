@@ -429,8 +429,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale: float 
 
     `q` has shape (sequences, q_heads, head_dim), head_dim at most 256; the caches and `block_table` are those of
     `append_kv`, with `q_heads` a multiple of the cache's heads. Sequence `s` looks at its first `seq_lens[s]` (int32)
-    tokens, or the last `window` of them when `window` is positive. A sequence of length zero gives zeros, and so does
-    a row whose weights are all zero. What the cache holds past a sequence's length or in front of its window doesn't
+    tokens, or the last `window` of them when `window` is positive. `o` may be `q`. A sequence of length zero gives
+    zeros, and so does a row whose weights are all zero. What the cache holds past a sequence's length or in front of its window doesn't
     matter; an infinite value among those that do can make its column NaN.
 
     With `return_lse=True`, also returns the float32 log-sum-exp of the scaled scores, shape (sequences, q_heads):

@@ -273,7 +273,8 @@ int enc_append_kv(const enc_paged_cache *cache, const enc_append_args *args, int
  * them when window > 0), with head h reading kv head h / (q_heads / kv_heads).  Statistics and sums in float32.  A row
  * without keys (length zero), or whose weights sum to zero, is zero with lse -inf.  lse: float32 [num_seqs, q_heads] or
  * NULL.  Cache contents past a sequence's length or in front of its window are never used.
- * q, o: [num_seqs, q_heads, head_dim] with strides per sequence and head; all of `dtype`; head_dim <= 256.
+ * q, o: [num_seqs, q_heads, head_dim] with strides per sequence and head; all of `dtype`; head_dim <= 256.  o may be q
+ * itself: a row's queries are read by the CTAs that write it, or before the launch that joins its pieces.
  * The keys of all sequences and heads are dealt out evenly over the GPU, whatever their lengths: the schedule is computed
  * on the device from seq_lens, so a captured launch follows the lengths it finds.  Pieces that do not finish a row go
  * through `work`, a buffer of at least enc_paged_attention_work_bytes() bytes, 16-byte aligned, whose contents need

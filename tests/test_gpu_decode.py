@@ -455,6 +455,28 @@ def test_attention_strided_arguments():
     enceladus.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("lens", [[130, 0, 1, 200], [20_000, 3, 0, 9_999]], ids=str)
+@pytest.mark.parametrize("variant", [None, *range(2)])
+def test_attention_output_over_the_queries(dtype, lens, variant):
+    """o may be q, for rows of one piece, of many and of none: the same bits as with an output of its own."""
+    q, kc, vc, table = make_attention(dtype, lens, heads=(12, 2), dim=64, garbage=0.0)
+    ops.paged_attention_kernel.variant = variant
+    try:
+        want = ops.paged_attention(q, kc, vc, table, ints(lens))
+        assert ops.paged_attention(q, kc, vc, table, ints(lens), o=q) is q
+    finally:
+        ops.paged_attention_kernel.variant = None
+    enceladus.synchronize()
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_attention_scales_of_any_sign(dtype, scale):
+    check_attention(dtype, [300, 0, 17, 900], scale=scale, dim=128)
+
+
 def test_attention_out_of_range_is_reported():
     q, kc, vc, table = make_attention(BF16, [100, 40], dim=64)
     for lens, page in (([8 * 16 + 1, 1], None), ([-1, 1], None), ([2**31 - 1, 1], None), ([100, 40], -1), ([100, 40], kc.shape[0])):
